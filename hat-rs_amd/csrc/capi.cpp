@@ -13,6 +13,7 @@
 #include "gpu.h"
 #include "hip_rt.h"
 #include "image.h"
+#include "ops.h"
 #include "tile.h"
 #include "kargs.h"
 #include "weights.h"
@@ -434,6 +435,40 @@ int hat_op_ocab(const float* x, float* out, int hp, int wp, int c, int heads, in
     return guard([&] {
         hat::op_ocab(x, out, hp, wp, c, heads, mlp_ratio, n1w, n1b, qkv_w, qkv_b, proj_w, proj_b, table,
                      n2w, n2b, fc1_w, fc1_b, fc2_w, fc2_b, iters, ms, attn_ms);
+        return 0;
+    });
+}
+
+int hat_op_rotary(const hat_rotary* a, void* stream)
+{
+    return guard([&] {
+        hat::op_rotary(a, stream);
+        return 0;
+    });
+}
+
+size_t hat_op_attention_workspace(const hat_attention* a)
+{
+    size_t n = (size_t)-1;
+    guard([&] {
+        n = hat::op_attention_workspace(a);
+        return 0;
+    });
+    return n;
+}
+
+int hat_op_attention(const hat_attention* a, void* stream)
+{
+    return guard([&] {
+        hat::op_attention(a, stream);
+        return 0;
+    });
+}
+
+int hat_op_residual_norm(const hat_residual_norm* a, void* stream)
+{
+    return guard([&] {
+        hat::op_residual_norm(a, stream);
         return 0;
     });
 }

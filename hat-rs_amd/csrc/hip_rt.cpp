@@ -35,6 +35,15 @@ const std::vector<std::string>& required_kernels()
         "hat_convwino_cab1_180", "hat_convwino_cab2_180", "hat_convw_n9_resid",
         "hat_convw_n4_store",  "hat_convw_n8_shuffle", "hat_convw_n6_resid", "hat_convw_n6_colsum", "hat_layernorm",       "hat_pre",  "hat_absmax", "hat_scale",             "hat_colsum_reduce",  "hat_se_gate",
         "hat_copy",
+        "hat_rotary_f32_v4", "hat_rotary_f32_v2", "hat_rotary_f32_v1", "hat_rotary_f16_v8", "hat_rotary_f16_v4",
+        "hat_rotary_f16_v1", "hat_rotary_bf16_v8", "hat_rotary_bf16_v4", "hat_rotary_bf16_v1",
+        "hat_attnseq_rows_f32", "hat_attnseq_rows_f16", "hat_attnseq_rows_bf16",
+        "hat_resnorm_f32_16", "hat_resnorm_f32_64", "hat_resnorm_f32_256", "hat_resnorm_f32_1024",
+        "hat_resnorm_f32_64e", "hat_resnorm_f32_1024e",
+        "hat_resnorm_f16_16", "hat_resnorm_f16_64", "hat_resnorm_f16_256", "hat_resnorm_f16_1024",
+        "hat_resnorm_f16_64e", "hat_resnorm_f16_1024e",
+        "hat_resnorm_bf16_16", "hat_resnorm_bf16_64", "hat_resnorm_bf16_256", "hat_resnorm_bf16_1024",
+        "hat_resnorm_bf16_64e", "hat_resnorm_bf16_1024e",
     };
     return k;
 }
@@ -104,6 +113,8 @@ Runtime::Runtime()
     sym(l, api_.Init, "hipInit");
     sym(l, api_.GetDeviceCount, "hipGetDeviceCount");
     sym(l, api_.SetDevice, "hipSetDevice");
+    sym(l, api_.GetDevice, "hipGetDevice");
+    sym(l, api_.StreamGetDevice, "hipStreamGetDevice");
     sym(l, api_.DeviceSynchronize, "hipDeviceSynchronize");
     sym(l, api_.GetErrorString, "hipGetErrorString");
     sym(l, api_.DeviceGetName, "hipDeviceGetName");
@@ -190,6 +201,18 @@ int Runtime::cu_count() const
     int v = 0;
     api_.DeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, 0);
     return v;
+}
+
+DeviceScope::DeviceScope()
+{
+    const HipApi& api = Runtime::get().api();
+    Runtime::get().check(api.GetDevice(&before_), "hipGetDevice");
+    if (before_ != 0) Runtime::get().check(api.SetDevice(0), "hipSetDevice(0)");
+}
+
+DeviceScope::~DeviceScope()
+{
+    if (before_ != 0) Runtime::get().api().SetDevice(before_);
 }
 
 void* Runtime::alloc(size_t bytes)
@@ -302,8 +325,9 @@ void launch_raw(hipStream_t stream, const char* name, unsigned gx, unsigned gy, 
     const HipApi& api = rt.api();
     hipFunction_t f = rt.fn(name);
     if (gx == 0 || gy == 0 || gz == 0) return;
-    // The kernarg segment holds exactly the argument struct.
-    alignas(16) unsigned char buf[512];
+    // The kernarg segment holds exactly the argument struct (at most RotaryArgs with
+    // its table of frequencies).
+    alignas(16) unsigned char buf[2048];
     if (size > sizeof buf) throw Error("kernel argument block too large");
     memcpy(buf, args, size);
     size_t sz = size;

@@ -28,6 +28,8 @@ struct HipApi {
     hipError_t (*Init)(unsigned int);
     hipError_t (*GetDeviceCount)(int*);
     hipError_t (*SetDevice)(int);
+    hipError_t (*GetDevice)(int*);
+    hipError_t (*StreamGetDevice)(hipStream_t, hipDevice_t*);
     hipError_t (*DeviceSynchronize)();
     const char* (*GetErrorString)(hipError_t);
     hipError_t (*DeviceGetName)(char*, int, int);
@@ -89,6 +91,18 @@ private:
     std::vector<std::string> names_;
     void* scratch_ = nullptr;
     size_t scratch_bytes_ = 0;
+};
+
+// Makes device 0, the module's, current for a scope and the caller's again behind
+// it: an operator may be called by a thread that works on another device.
+class DeviceScope {
+public:
+    DeviceScope();
+    ~DeviceScope();
+    DeviceScope(const DeviceScope&) = delete;
+
+private:
+    int before_ = 0;
 };
 
 // True if the HIP runtime library can be opened and reports a device. Never

@@ -365,4 +365,57 @@ struct ReduceArgs {
     int nrows, C, stride, rows_per;
 };
 
+// ---- operators on device tensors (rotary.hip, attnseq.hip, resnorm.hip) ------
+// Strides are in elements; the last axis of every tensor has stride 1.
+
+#define ROT_AXES 4
+#define ROT_PAIRS 128        // rotated pairs of a head at most (head_dim 256)
+
+// Rotary positions of up to two tensors [batch][token][head][dim] (q and k).
+struct RotaryArgs {
+    const void* x[2];
+    void* y[2];
+    long long xb[2], xt[2], xh[2], yb[2], yt[2], yh[2];
+    int heads[2];            // heads[1] = 0: one tensor
+    const int* pos;          // [batch][token][axis]
+    long long pb, pt, pa;
+    long long tokens, blocks;  // tokens per batch entry; blocks of `per` tokens each
+    int batch, per, dim, pairs;
+    int chunks;              // work items of a head: rotated, then copied ones
+    int neighbours;          // pairs (2i, 2i + 1) instead of (i, i + pairs)
+    int ends[ROT_AXES];      // pair i belongs to the first axis with i < ends[axis]
+    float inv_chunks, inv_items, inv_pairs;  // 1 / chunks, 1 / (chunks * heads), 1 / pairs
+    double turn[ROT_PAIRS];  // revolutions per unit of position (negative: inverse)
+};
+
+// Attention over sequences: sequence s's tokens are rows cu[s] .. cu[s + 1) of a
+// packed tensor, or entry s of a batch with lens[s] (or all) of its tokens in use.
+struct SeqAttnArgs {
+    const void *q, *k, *v;
+    void* o;
+    long long qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
+    const int *cu_q, *cu_k, *q_lens, *k_lens, *prefix;
+    const float* slopes;     // [q_heads] or null
+    const int *pos_q, *pos_k;
+    long long pqb, pqt, pqa, pkb, pkt, pka;
+    int n_seq, q_heads, kv_heads, group, dim, axes;
+    int q_tokens, k_tokens;  // of a batch entry, or of the packed tensor
+    int causal;
+    float scale;             // scores = scale * q . k
+    float cap, inv_cap;      // cap > 0: cap * tanh(scores * inv_cap)
+};
+
+enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
+
+// x' = x + scale * gate * Npost(y), h = Npre(x'), row by row.
+struct ResNormArgs {
+    const void *x, *y, *gate;  // y, gate: may be null
+    void *xo, *h;              // either may be null
+    const float *post_w, *post_b, *pre_w, *pre_b;  // null: ones, zeros
+    long long xs, ys, gs, xos, hs;                 // row strides
+    long long rows, rows_per_gate;
+    int width, post, pre;
+    float scale, post_eps, pre_eps;
+};
+
 }  // namespace hatk

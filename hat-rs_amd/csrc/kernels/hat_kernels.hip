@@ -13,3 +13,6 @@
 #include "convwino.hip"
 #include "misc.hip"
 #include "convfirst.hip"
+#include "rotary.hip"
+#include "attnseq.hip"
+#include "resnorm.hip"

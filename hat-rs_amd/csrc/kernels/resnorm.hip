@@ -1,0 +1,143 @@
+// The join of a block's output with the residual stream and the norm behind it:
+//   x' = x + scale * gate * Npost(y),  h = Npre(x'),
+// Npost and Npre each LayerNorm, RMSNorm or nothing, the gate a row of its own for
+// every rows_per_gate rows. y may be missing (x' = x), x' or h may be left out.
+//
+// What bounds it: HBM, x and y read once, x' and h written once. A row's values stay
+// in registers between the reading and the second norm, so both norms' sums (a mean,
+// then the sum of squared differences from it) run over registers; h is formed from
+// x' before its rounding. A row takes 16, 64, 256 or 1024 threads by its width.
+#include "types.h"
+
+using namespace hatk;
+
+// The sum over a row's TPR threads, the same in each, added in a fixed order.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* lds)
+{
+#pragma unroll
+    for (int o = TPR < 64 ? TPR / 2 : 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (TPR > 64) {
+        __syncthreads();  // the last sum's values have been read
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) v += lds[w];
+    }
+    return v;
+}
+
+// v = N(v) over the row's p.width values.
+template <int TPR, int V, int NV>
+__device__ __forceinline__ void row_norm(float (&v)[NV][V], int kind, const float* w, const float* b, float eps,
+                                         int width, int t, float* lds)
+{
+    float mean = 0.0f;
+    if (kind == NORM_LAYER) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += v[i][j];  // zeros past the width
+        mean = row_sum<TPR>(s, lds) / (float)width;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if ((i * TPR + t) * V < width) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[i][j] -= mean;
+                q = __builtin_fmaf(v[i][j], v[i][j], q);
+            }
+        }
+    }
+    const float r = 1.0f / sqrtf(row_sum<TPR>(q, lds) / (float)width + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * V;
+        if (c < width) {
+            float f[V], a[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = 1.0f, a[j] = 0.0f;
+            if (w) load_vec<float, V>(w + c, f);
+            if (b) load_vec<float, V>(b + c, a);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][j] = __builtin_fmaf(v[i][j] * r, f[j], a[j]);
+        }
+    }
+}
+
+// THREADS a block, TPR of them a row, NV vectors of V elements a thread.
+template <class T, int THREADS, int TPR, int V, int NV>
+__device__ __forceinline__ void resnorm_body(const ResNormArgs& p)
+{
+    __shared__ float lds[THREADS / 64];
+    const int t = threadIdx.x % TPR;
+    const long long row = (long long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+    if (row >= p.rows) return;  // whole rows leave; with more than a wave a row, whole blocks
+    float v[NV][V];
+    if (p.y) {
+        const T* y = (const T*)p.y + row * p.ys;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+            if ((i * TPR + t) * V < p.width) load_vec<T, V>(y + (i * TPR + t) * V, v[i]);
+        }
+        if (p.post != NORM_NONE) row_norm<TPR, V, NV>(v, p.post, p.post_w, p.post_b, p.post_eps, p.width, t, lds);
+    }
+    const T* x = (const T*)p.x + row * p.xs;
+    const T* g = p.gate ? (const T*)p.gate + row / p.rows_per_gate * p.gs : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * V;
+        float u[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = 0.0f;
+        if (c < p.width) {
+            load_vec<T, V>(x + c, u);
+            if (p.y) {
+                float f[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[j] = 1.0f;
+                if (g) load_vec<T, V>(g + c, f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(p.scale * f[j], v[i][j], u[j]);
+            }
+            if (p.xo) store_vec<T, V>((T*)p.xo + row * p.xos + c, u);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = u[j];
+    }
+    if (!p.h) return;
+    if (p.pre != NORM_NONE) row_norm<TPR, V, NV>(v, p.pre, p.pre_w, p.pre_b, p.pre_eps, p.width, t, lds);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * V;
+        if (c < p.width) store_vec<T, V>((T*)p.h + row * p.hs + c, v[i]);
+    }
+}
+
+#define RESNORM_INST(NAME, T, THREADS, TPR, V, NV) \
+    extern "C" __global__ __launch_bounds__(THREADS) void NAME(ResNormArgs p) { resnorm_body<T, THREADS, TPR, V, NV>(p); }
+
+RESNORM_INST(hat_resnorm_f32_16, float, 256, 16, 4, 3)
+RESNORM_INST(hat_resnorm_f32_64, float, 256, 64, 4, 4)
+RESNORM_INST(hat_resnorm_f32_256, float, 256, 256, 4, 4)
+RESNORM_INST(hat_resnorm_f32_1024, float, 1024, 1024, 4, 4)
+RESNORM_INST(hat_resnorm_f32_64e, float, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_f32_1024e, float, 1024, 1024, 1, 16)
+RESNORM_INST(hat_resnorm_f16_16, f16, 256, 16, 8, 2)
+RESNORM_INST(hat_resnorm_f16_64, f16, 256, 64, 8, 4)
+RESNORM_INST(hat_resnorm_f16_256, f16, 256, 256, 8, 4)
+RESNORM_INST(hat_resnorm_f16_1024, f16, 1024, 1024, 8, 2)
+RESNORM_INST(hat_resnorm_f16_64e, f16, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_f16_1024e, f16, 1024, 1024, 1, 16)
+RESNORM_INST(hat_resnorm_bf16_16, bf16, 256, 16, 8, 2)
+RESNORM_INST(hat_resnorm_bf16_64, bf16, 256, 64, 8, 4)
+RESNORM_INST(hat_resnorm_bf16_256, bf16, 256, 256, 8, 4)
+RESNORM_INST(hat_resnorm_bf16_1024, bf16, 1024, 1024, 8, 2)
+RESNORM_INST(hat_resnorm_bf16_64e, bf16, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_bf16_1024e, bf16, 1024, 1024, 1, 16)

@@ -1,0 +1,356 @@
+#include "ops.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "hip_rt.h"
+#include "kargs.h"
+
+namespace hat {
+
+using namespace hatk;
+
+namespace {
+
+constexpr long long MAX_STRIDE = 1ll << 40;  // elements: every offset stays far inside 64 bits
+constexpr double LOG2E = 1.4426950408889634;
+
+size_t element(int dtype) { return dtype == HAT_F32 ? 4 : 2; }
+
+const char* type_name(int dtype) { return dtype == HAT_F32 ? "f32" : dtype == HAT_F16 ? "f16" : "bf16"; }
+
+void check_dtype(const char* op, int dtype)
+{
+    if (dtype != HAT_F32 && dtype != HAT_F16 && dtype != HAT_BF16)
+        throw Error(std::string(op) + ": type " + std::to_string(dtype) + " is none of HAT_F32, HAT_F16, HAT_BF16");
+}
+
+void check_range(const char* op, const char* what, long long v, long long lo, long long hi)
+{
+    if (v < lo || v > hi)
+        throw Error(std::string(op) + ": " + what + " " + std::to_string(v) + " is out of range (" + std::to_string(lo) +
+                    " to " + std::to_string(hi) + ")");
+}
+
+void check_pointer(const char* op, const char* what, const void* p, size_t align)
+{
+    if (!p) throw Error(std::string(op) + ": " + what + " is null");
+    if ((uintptr_t)p % align) throw Error(std::string(op) + ": " + what + " is not aligned to its elements");
+}
+
+void check_stride(const char* op, const char* what, long long v)
+{
+    if (v < 0 || v > MAX_STRIDE) throw Error(std::string(op) + ": " + what + " has a stride of " + std::to_string(v));
+}
+
+void check_heads(const char* op, const char* what, const hat_heads& t, int dtype)
+{
+    check_pointer(op, what, t.data, element(dtype));
+    check_stride(op, what, t.batch_stride);
+    check_stride(op, what, t.token_stride);
+    check_stride(op, what, t.head_stride);
+}
+
+// An output's rows lie apart: an axis of more than one entry moves at least a row on.
+void check_rows_apart(const char* op, const char* what, const hat_heads& t, long long batch, long long tokens, int heads, int dim)
+{
+    if ((batch > 1 && t.batch_stride < dim) || (tokens > 1 && t.token_stride < dim) || (heads > 1 && t.head_stride < dim))
+        throw Error(std::string(op) + ": " + what + " has rows on top of one another");
+}
+
+void check_replaces(const char* op, const char* what, const hat_heads& in, const hat_heads& out)
+{
+    if (in.data == out.data && (in.batch_stride != out.batch_stride || in.token_stride != out.token_stride ||
+                                in.head_stride != out.head_stride))
+        throw Error(std::string(op) + ": " + what + " overlaps its input with other strides");
+}
+
+void check_positions(const char* op, const hat_positions& p)
+{
+    check_pointer(op, "positions", p.data, 4);
+    check_stride(op, "positions", p.batch_stride);
+    check_stride(op, "positions", p.token_stride);
+    check_stride(op, "positions", p.axis_stride);
+}
+
+// The caller's stream, refused where it is another device's.
+hipStream_t check_stream(const char* op, void* stream)
+{
+    if (stream) {
+        hipDevice_t dev = -1;
+        const Runtime& rt = Runtime::get();
+        rt.check(rt.api().StreamGetDevice((hipStream_t)stream, &dev), "hipStreamGetDevice");
+        if (dev != 0) throw Error(std::string(op) + ": the stream belongs to device " + std::to_string(dev) + ", not 0");
+    }
+    return (hipStream_t)stream;
+}
+
+// Whether rows at these offsets from data can be moved `bytes` at a time.
+bool aligned(const hat_heads& t, int dtype, size_t bytes)
+{
+    const size_t e = element(dtype);
+    return ((uintptr_t)t.data | (size_t)t.batch_stride * e | (size_t)t.token_stride * e | (size_t)t.head_stride * e) % bytes == 0;
+}
+
+unsigned grid_of(const char* op, long long blocks)
+{
+    if (blocks > 0x7fffffffll) throw Error(std::string(op) + ": too large");
+    return (unsigned)blocks;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+
+void op_rotary(const hat_rotary* a, void* stream)
+{
+    const char* op = "rotary";
+    if (!a) throw Error("rotary: null argument");
+    check_dtype(op, a->dtype);
+    check_range(op, "head_dim", a->head_dim, 1, 2 * ROT_PAIRS);
+    check_range(op, "axes", a->axes, 1, ROT_AXES);
+    check_range(op, "batch", a->batch, 0, 1 << 30);
+    check_range(op, "tokens", a->tokens, 0, 1ll << 31);
+    check_range(op, "q_heads", a->q_heads, 1, 1 << 12);
+    check_range(op, "k_heads", a->k_heads, a->k.data || a->k_out.data ? 1 : 0, 1 << 12);
+    if (!(a->base > 0.0) || !std::isfinite(a->base)) throw Error("rotary: base must be positive");
+    int pairs = 0;
+    RotaryArgs p{};
+    for (int x = 0; x < ROT_AXES; ++x) {
+        if (x < a->axes) {
+            check_range(op, "section", a->sections[x], 0, ROT_PAIRS);
+            pairs += a->sections[x];
+        }
+        p.ends[x] = pairs;
+    }
+    if (pairs < 1 || 2 * pairs > a->head_dim)
+        throw Error("rotary: sections of " + std::to_string(pairs) + " pairs do not fit a head_dim of " +
+                    std::to_string(a->head_dim));
+    if (a->batch == 0 || a->tokens == 0) return;
+    const bool two = a->k.data || a->k_out.data;
+    const hat_heads* in[2] = {&a->q, &a->k};
+    const hat_heads* out[2] = {&a->q_out, &a->k_out};
+    const int heads[2] = {a->q_heads, two ? a->k_heads : 0};
+    bool in_place = true;
+    for (int w = 0; w < (two ? 2 : 1); ++w) {
+        check_heads(op, w ? "k" : "q", *in[w], a->dtype);
+        check_heads(op, w ? "k_out" : "q_out", *out[w], a->dtype);
+        check_rows_apart(op, w ? "k_out" : "q_out", *out[w], a->batch, a->tokens, heads[w], a->head_dim);
+        check_replaces(op, w ? "k_out" : "q_out", *in[w], *out[w]);
+        in_place = in_place && in[w]->data == out[w]->data;
+    }
+    check_positions(op, a->pos);
+
+    // The widest move that every row, the pairs' halves and the copied rest allow.
+    // 57600 tokens of 24 heads of 72 in f16, 28 pairs (8 bytes): see rotary.hip.
+    const int size = (int)element(a->dtype);
+    const int widths[2] = {16 / size, 8 / size};
+    int V = 1;
+    for (int v : widths) {
+        bool ok = a->head_dim % v == 0 && (a->neighbours ? 2 * pairs : pairs) % v == 0;
+        for (int w = 0; ok && w < (two ? 2 : 1); ++w)
+            ok = aligned(*in[w], a->dtype, v * size) && aligned(*out[w], a->dtype, v * size);
+        if (ok) {
+            V = v;
+            break;
+        }
+    }
+    for (int w = 0; w < 2; ++w) {
+        p.x[w] = in[w]->data, p.y[w] = out[w]->data;
+        p.xb[w] = in[w]->batch_stride, p.xt[w] = in[w]->token_stride, p.xh[w] = in[w]->head_stride;
+        p.yb[w] = out[w]->batch_stride, p.yt[w] = out[w]->token_stride, p.yh[w] = out[w]->head_stride;
+        p.heads[w] = heads[w];
+    }
+    p.pos = a->pos.data, p.pb = a->pos.batch_stride, p.pt = a->pos.token_stride, p.pa = a->pos.axis_stride;
+    p.tokens = a->tokens, p.batch = a->batch;
+    p.dim = a->head_dim, p.pairs = pairs, p.neighbours = a->neighbours != 0;
+    const int turned = a->neighbours && V > 1 ? 2 * pairs / V : pairs / V;
+    const int rest = in_place ? 0 : (a->head_dim - 2 * pairs) / V;  // in place they are there already
+    p.chunks = turned + rest;
+    const int items = p.chunks * (heads[0] + heads[1]);
+    int n = 0;
+    for (int x = 0; x < a->axes; ++x)
+        for (int i = 0; i < a->sections[x]; ++i, ++n) {
+            const double ladder = a->joint ? (double)n / pairs : (double)i / a->sections[x];
+            const double turn = std::pow(a->base, -ladder) / (2.0 * M_PI);
+            p.turn[n] = a->inverse ? -turn : turn;
+        }
+    // Tokens a block: about eight items a thread, fewer while the grid would not
+    // fill the device, and within the angles' LDS and div_small's range.
+    const long long all = a->tokens * a->batch;
+    int per = std::max(1, std::min({2048 / items, 4096 / pairs, 64}));
+    while (per > 1 && all / per < 2048) per = (per + 1) / 2;
+    p.per = per;
+    p.blocks = (all + per - 1) / per;
+    p.inv_chunks = 1.0f / p.chunks, p.inv_items = 1.0f / items, p.inv_pairs = 1.0f / pairs;
+    if ((long long)per * items >= 1 << 20) throw Error("rotary: too many heads");
+    const DeviceScope scope;
+    hipStream_t s = check_stream(op, stream);
+    const std::string name = std::string("hat_rotary_") + type_name(a->dtype) + "_v" + std::to_string(V);
+    launch(s, name.c_str(), grid_of(op, p.blocks), 1, 1, 256, p);
+}
+
+// ---------------------------------------------------------------------------
+
+namespace {
+
+void check_attention(const hat_attention* a)
+{
+    const char* op = "attention";
+    if (!a) throw Error("attention: null argument");
+    check_dtype(op, a->dtype);
+    check_range(op, "head_dim", a->head_dim, 1, 128);
+    check_range(op, "n_seq", a->n_seq, 0, 1 << 24);
+    check_range(op, "kv_heads", a->kv_heads, 1, 1 << 12);
+    check_range(op, "q_heads", a->q_heads, 1, 1 << 12);
+    if (a->q_heads % a->kv_heads)
+        throw Error("attention: " + std::to_string(a->q_heads) + " query heads do not divide over " +
+                    std::to_string(a->kv_heads) + " key heads");
+    check_range(op, "q_tokens", a->q_tokens, 0, (1ll << 31) - 1024);
+    check_range(op, "k_tokens", a->k_tokens, 0, (1ll << 31) - 1024);
+    if (!std::isfinite(a->scale)) throw Error("attention: scale must be finite");
+    if (!(a->cap >= 0.0f) || !std::isfinite(a->cap)) throw Error("attention: cap must be 0 or positive");
+    if ((a->cu_q && a->q_lens) || (a->cu_k && a->k_lens))
+        throw Error("attention: a packed tensor has offsets, not lengths");
+    if (a->prefix && !a->causal) throw Error("attention: a prefix belongs to the causal mask");
+    // (tensors without tokens may have no address)
+    if (a->q_tokens && a->k_tokens && (a->pos_q.data != nullptr) != (a->pos_k.data != nullptr))
+        throw Error("attention: positions of queries and keys go together");
+    if (a->pos_q.data && !a->slopes) throw Error("attention: positions without slopes");
+    if (a->pos_q.data) check_range(op, "axes", a->axes, 1, 4);
+}
+
+}  // namespace
+
+size_t op_attention_workspace(const hat_attention* a)
+{
+    check_attention(a);
+    return 0;
+}
+
+void op_attention(const hat_attention* a, void* stream)
+{
+    const char* op = "attention";
+    check_attention(a);
+    if (a->n_seq == 0 || a->q_tokens == 0) return;
+    check_heads(op, "q", a->q, a->dtype);
+    check_heads(op, "out", a->out, a->dtype);
+    check_rows_apart(op, "out", a->out, a->cu_q ? 1 : a->n_seq, a->q_tokens, a->q_heads, a->head_dim);
+    check_replaces(op, "out", a->q, a->out);
+    if (a->k_tokens) {
+        check_heads(op, "k", a->k, a->dtype);
+        check_heads(op, "v", a->v, a->dtype);
+        if (a->pos_q.data) {
+            check_positions(op, a->pos_q);
+            check_positions(op, a->pos_k);
+        }
+    }
+    for (const void* i : {(const void*)a->cu_q, (const void*)a->cu_k, (const void*)a->q_lens, (const void*)a->k_lens,
+                          (const void*)a->prefix, (const void*)a->slopes})
+        if (i) check_pointer(op, "an int32 or fp32 argument", i, 4);
+    SeqAttnArgs p{};
+    p.q = a->q.data, p.k = a->k.data, p.v = a->v.data, p.o = a->out.data;
+    p.qb = a->q.batch_stride, p.qt = a->q.token_stride, p.qh = a->q.head_stride;
+    p.kb = a->k.batch_stride, p.kt = a->k.token_stride, p.kh = a->k.head_stride;
+    p.vb = a->v.batch_stride, p.vt = a->v.token_stride, p.vh = a->v.head_stride;
+    p.ob = a->out.batch_stride, p.ot = a->out.token_stride, p.oh = a->out.head_stride;
+    p.cu_q = a->cu_q, p.cu_k = a->cu_k, p.q_lens = a->q_lens, p.k_lens = a->k_lens, p.prefix = a->prefix;
+    p.slopes = a->slopes;
+    if (a->pos_q.data && a->k_tokens) {
+        p.pos_q = a->pos_q.data, p.pos_k = a->pos_k.data, p.axes = a->axes;
+        p.pqb = a->pos_q.batch_stride, p.pqt = a->pos_q.token_stride, p.pqa = a->pos_q.axis_stride;
+        p.pkb = a->pos_k.batch_stride, p.pkt = a->pos_k.token_stride, p.pka = a->pos_k.axis_stride;
+    }
+    p.n_seq = a->n_seq, p.q_heads = a->q_heads, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads;
+    p.dim = a->head_dim;
+    p.q_tokens = (int)a->q_tokens, p.k_tokens = (int)a->k_tokens;
+    p.causal = a->causal != 0;
+    p.scale = a->scale;
+    p.cap = a->cap, p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
+    const DeviceScope scope;
+    hipStream_t s = check_stream(op, stream);
+    const long long rows = a->q_tokens * a->q_heads * (a->cu_q ? 1 : a->n_seq);
+    launch(s, (std::string("hat_attnseq_rows_") + type_name(a->dtype)).c_str(), grid_of(op, (rows + 3) / 4), 1, 1, 256, p);
+}
+
+// ---------------------------------------------------------------------------
+
+void op_residual_norm(const hat_residual_norm* a, void* stream)
+{
+    const char* op = "residual_norm";
+    if (!a) throw Error("residual_norm: null argument");
+    check_dtype(op, a->dtype);
+    check_range(op, "width", a->width, 1, 16384);
+    check_range(op, "rows", a->rows, 0, 1ll << 40);
+    check_range(op, "post", a->post, HAT_NORM_NONE, HAT_NORM_RMS);
+    check_range(op, "pre", a->pre, HAT_NORM_NONE, HAT_NORM_RMS);
+    if (!a->y && (a->post != HAT_NORM_NONE || a->gate)) throw Error("residual_norm: a norm or a gate of no y");
+    if (a->post == HAT_NORM_NONE && (a->post_w || a->post_b)) throw Error("residual_norm: weights of no norm");
+    if (a->pre == HAT_NORM_NONE && (a->pre_w || a->pre_b)) throw Error("residual_norm: weights of no norm");
+    if (!std::isfinite(a->scale) || !(a->post_eps >= 0.0f) || !(a->pre_eps >= 0.0f))
+        throw Error("residual_norm: scale must be finite, eps 0 or positive");
+    if (a->gate) check_range(op, "rows_per_gate", a->rows_per_gate, 1, 1ll << 40);
+    if (a->rows == 0) return;  // tensors without rows may have no address
+    if (!a->x_out && !a->h) throw Error("residual_norm: no output");
+    const size_t e = element(a->dtype);
+    const struct {
+        const char* what;
+        const void* p;
+        long long stride;
+        bool out;
+    } rows[] = {{"x", a->x, a->x_stride, false},
+                {"y", a->y, a->y_stride, false},
+                {"gate", a->gate, a->gate_stride, false},
+                {"x_out", a->x_out, a->x_out_stride, true},
+                {"h", a->h, a->h_stride, true}};
+    if (!a->x) throw Error("residual_norm: x is null");
+    bool wide = a->width % (16 / (int)e) == 0;
+    for (const auto& r : rows) {
+        if (!r.p) continue;
+        check_pointer(op, r.what, r.p, e);
+        check_stride(op, r.what, r.stride);
+        if (r.out && a->rows > 1 && r.stride < a->width)
+            throw Error(std::string("residual_norm: ") + r.what + " has rows on top of one another");
+        wide = wide && ((uintptr_t)r.p | (size_t)r.stride * e) % 16 == 0;
+    }
+    for (int i = 0; i < 2; ++i)
+        for (int o = 3; o < 5; ++o)
+            if (rows[i].p && rows[i].p == rows[o].p && rows[i].stride != rows[o].stride && a->rows > 1)
+                throw Error(std::string("residual_norm: ") + rows[o].what + " overlaps its input with other strides");
+    if (a->x_out && a->x_out == a->h) throw Error("residual_norm: x_out and h are the same rows");
+    for (const float* w : {a->post_w, a->post_b, a->pre_w, a->pre_b}) {
+        if (!w) continue;
+        check_pointer(op, "a norm's weight", w, 4);
+        wide = wide && (uintptr_t)w % 16 == 0;
+    }
+    ResNormArgs p{};
+    p.x = a->x, p.y = a->y, p.gate = a->gate, p.xo = a->x_out, p.h = a->h;
+    p.post_w = a->post_w, p.post_b = a->post_b, p.pre_w = a->pre_w, p.pre_b = a->pre_b;
+    p.xs = a->x_stride, p.ys = a->y_stride, p.gs = a->gate_stride, p.xos = a->x_out_stride, p.hs = a->h_stride;
+    p.rows = a->rows, p.rows_per_gate = a->gate ? a->rows_per_gate : 1;
+    p.width = a->width, p.post = a->post, p.pre = a->pre;
+    p.scale = a->scale, p.post_eps = a->post_eps, p.pre_eps = a->pre_eps;
+    // The fewest threads a row whose registers hold it.
+    const int W = a->width;
+    const char* form;
+    int per, threads = 256;
+    if (!wide)
+        form = W <= 1024 ? "64e" : "1024e", per = W <= 1024 ? 4 : 1;
+    else if (W <= (a->dtype == HAT_F32 ? 192 : 256))
+        form = "16", per = 16;
+    else if (W <= (a->dtype == HAT_F32 ? 1024 : 2048))
+        form = "64", per = 4;
+    else if (W <= (a->dtype == HAT_F32 ? 4096 : 8192))
+        form = "256", per = 1;
+    else
+        form = "1024", per = 1;
+    if (form[0] == '1' && form[1] == '0') threads = 1024;
+    const DeviceScope scope;
+    hipStream_t s = check_stream(op, stream);
+    const std::string name = std::string("hat_resnorm_") + type_name(a->dtype) + "_" + form;
+    launch(s, name.c_str(), grid_of(op, (a->rows + per - 1) / per), 1, 1, threads, p);
+}
+
+}  // namespace hat

@@ -36,6 +36,42 @@ class Tiling(C.Structure):
     _fields_ = [(n, C.c_size_t) for n in ("tile", "margin", "scale", "tiles", "largest_h", "largest_w")]
 
 
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_longlong), ("token_stride", C.c_longlong),
+                ("head_stride", C.c_longlong)]
+
+
+class Positions(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_longlong), ("token_stride", C.c_longlong),
+                ("axis_stride", C.c_longlong)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("q_heads", C.c_int), ("k_heads", C.c_int),
+                ("head_dim", C.c_int), ("axes", C.c_int), ("tokens", C.c_longlong), ("sections", C.c_int * 4),
+                ("joint", C.c_int), ("neighbours", C.c_int), ("inverse", C.c_int), ("base", C.c_double),
+                ("pos", Positions), ("q", Heads), ("q_out", Heads), ("k", Heads), ("k_out", Heads)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("n_seq", C.c_int), ("q_heads", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("axes", C.c_int), ("q_tokens", C.c_longlong), ("k_tokens", C.c_longlong),
+                ("q", Heads), ("k", Heads), ("v", Heads), ("out", Heads),
+                ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_lens", C.c_void_p), ("k_lens", C.c_void_p),
+                ("prefix", C.c_void_p), ("causal", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
+                ("slopes", C.c_void_p), ("pos_q", Positions), ("pos_k", Positions), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class ResidualNormArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("width", C.c_int), ("post", C.c_int), ("pre", C.c_int),
+                ("rows", C.c_longlong), ("rows_per_gate", C.c_longlong), ("x", C.c_void_p), ("y", C.c_void_p),
+                ("gate", C.c_void_p), ("x_out", C.c_void_p), ("h", C.c_void_p), ("x_stride", C.c_longlong),
+                ("y_stride", C.c_longlong), ("gate_stride", C.c_longlong), ("x_out_stride", C.c_longlong),
+                ("h_stride", C.c_longlong), ("post_w", C.c_void_p), ("post_b", C.c_void_p), ("pre_w", C.c_void_p),
+                ("pre_b", C.c_void_p), ("scale", C.c_float), ("post_eps", C.c_float), ("pre_eps", C.c_float)]
+
+
 class MemPlan(C.Structure):
     _fields_ = [(n, C.c_ulonglong) for n in ("activations", "weights", "base", "need", "avail")] + \
                [("have_avail", C.c_int)]
@@ -96,6 +132,10 @@ def lib():
                                    _f32p, _f32p, _f32p, _f32p, _f32p, C.c_int, _f32p, _f32p]),
         "hat_op_ocab": (C.c_int, [_f32p, _f32p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]
                         + [_f32p] * 13 + [C.c_int, _f32p, _f32p]),
+        "hat_op_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+        "hat_op_attention_workspace": (C.c_size_t, [C.POINTER(AttentionArgs)]),
+        "hat_op_attention": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+        "hat_op_residual_norm": (C.c_int, [C.POINTER(ResidualNormArgs), C.c_void_p]),
         "hat_device_alloc": (C.c_void_p, [C.c_size_t]),
         "hat_device_free": (C.c_int, [C.c_void_p]),
         "hat_memcpy_h2d": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
@@ -445,3 +485,246 @@ def profile_end():
         _check(L.hat_profile_get(i, buf, 128, C.byref(cnt), C.byref(tot)), "profile_get")
         out[buf.value.decode()] = (cnt.value, tot.value)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Operators on device tensors (include/hat.h). A device tensor is a DeviceArray or any
+# object with its five methods and attributes: data_ptr(), get_device() (0: the
+# library's device), stride() in elements, shape and dtype, as torch's tensors have.
+
+_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 3, "uint8": 4}
+_SIZES = {0: 4, 1: 2, 2: 2, 3: 4, 4: 1}
+_NORMS = {"none": 0, "layer": 1, "rms": 2}
+_dtype_codes = {}
+
+
+class DeviceArray:
+    """A contiguous device tensor of its own: a DeviceBuffer with a shape and a type
+    ("float32", "float16", "bfloat16", "int32", "uint8")."""
+
+    def __init__(self, shape, dtype, data=None):
+        self.shape, self.dtype = tuple(shape), dtype
+        count = 1
+        for n in self.shape:
+            count *= n
+        self.buffer = DeviceBuffer(max(4, count * _SIZES[_DTYPES[dtype]]))
+        if data is not None:
+            data = np.ascontiguousarray(data)
+            if data.nbytes != count * _SIZES[_DTYPES[dtype]]:
+                raise HatError(f"DeviceArray: {data.nbytes} bytes for a shape of {self.shape} in {dtype}")
+            if data.nbytes:
+                self.buffer.upload(data)
+
+    def data_ptr(self):
+        return self.buffer.ptr
+
+    def get_device(self):
+        return 0
+
+    def stride(self):
+        s, out = 1, []
+        for n in reversed(self.shape):
+            out.append(s)
+            s *= n
+        return tuple(reversed(out))
+
+    def numpy(self):
+        """A copy on the host; bfloat16 as its uint16 bits."""
+        kind = {"bfloat16": "uint16"}.get(self.dtype, self.dtype)
+        out = np.empty(self.shape, dtype=kind)
+        return self.buffer.download(out) if out.nbytes else out
+
+
+def _code(t, what):
+    """The type of a device tensor as the C ABI's number; refuses what is not on the device."""
+    d = t.dtype
+    c = _dtype_codes.get(d)
+    if c is None:
+        c = _DTYPES.get(str(d).replace("torch.", ""))
+        if c is None:
+            raise HatError(f"{what}: type {d} is not supported")
+        _dtype_codes[d] = c
+    if t.get_device() != 0:
+        raise HatError(f"{what}: not a tensor of device 0")
+    return c
+
+
+def _heads(t, what, code, lead=None):
+    """(Heads, batch, tokens, heads, dim) of [batch, token, head, dim] or [token, head, dim]."""
+    if _code(t, what) != code:
+        raise HatError(f"{what}: type {t.dtype} differs from the first tensor's")
+    shape, st = t.shape, t.stride()
+    if len(shape) not in (3, 4):
+        raise HatError(f"{what}: [batch, token, head, dim] or [token, head, dim] expected, not {tuple(shape)}")
+    if shape[-1] > 1 and st[-1] != 1:
+        raise HatError(f"{what}: the last axis must have stride 1")
+    if lead is not None and tuple(shape) != lead:
+        raise HatError(f"{what}: {tuple(shape)} where {lead} is expected")
+    if len(shape) == 4:
+        return Heads(t.data_ptr(), st[0], st[1], st[2]), shape[0], shape[1], shape[2], shape[3]
+    return Heads(t.data_ptr(), 0, st[0], st[1]), 1, shape[0], shape[1], shape[2]
+
+
+def _positions(t, what, batch, tokens):
+    """(Positions, axes) of int32 [token, axis], shared by the batch, or [batch, token, axis]."""
+    if _code(t, what) != 3:
+        raise HatError(f"{what}: int32 expected, not {t.dtype}")
+    shape, st = tuple(t.shape), t.stride()
+    if len(shape) == 2 and shape[0] == tokens:
+        return Positions(t.data_ptr(), 0, st[0], st[1]), shape[1]
+    if len(shape) == 3 and shape[:2] == (batch, tokens):
+        return Positions(t.data_ptr(), st[0], st[1], st[2]), shape[2]
+    raise HatError(f"{what}: {shape} is no [{tokens}, axis] or [{batch}, {tokens}, axis]")
+
+
+def _vector(t, what, code, n):
+    """The pointer of a contiguous vector of n values, or None."""
+    if t is None:
+        return None
+    if _code(t, what) != code or tuple(t.shape) != (n,) or (n > 1 and t.stride()[0] != 1):
+        raise HatError(f"{what}: {n} contiguous values of {'fp32' if code == 0 else 'int32'} expected")
+    return t.data_ptr()
+
+
+def op_rotary(q, k, pos, sections, base=10000.0, pairs="halves", joint=False, inverse=False, q_out=None, k_out=None,
+              stream=None):
+    """hat_op_rotary: turns q and k (None: q alone) by their tokens' positions, in place
+    where q_out / k_out are left out. pairs: "halves" or "neighbours"; stream: a
+    hipStream_t as an integer (torch's `cuda_stream`), None the default stream."""
+    a = RotaryArgs()
+    a.dtype = code = _code(q, "rotary: q")
+    a.q, a.batch, a.tokens, a.q_heads, a.head_dim = _heads(q, "rotary: q", code)
+    a.q_out = a.q if q_out is None else _heads(q_out, "rotary: q_out", code, tuple(q.shape))[0]
+    if k is not None:
+        a.k, b, t, a.k_heads, d = _heads(k, "rotary: k", code)
+        if (b, t, d) != (a.batch, a.tokens, a.head_dim):
+            raise HatError(f"rotary: k of {tuple(k.shape)} does not go with q of {tuple(q.shape)}")
+        a.k_out = a.k if k_out is None else _heads(k_out, "rotary: k_out", code, tuple(k.shape))[0]
+    elif k_out is not None:
+        raise HatError("rotary: k_out without k")
+    a.pos, axes = _positions(pos, "rotary: pos", a.batch, a.tokens)
+    if axes != len(sections) or not 1 <= axes <= 4:
+        raise HatError(f"rotary: {axes} axes of positions and {len(sections)} sections (1 to 4)")
+    if pairs not in ("halves", "neighbours"):
+        raise HatError(f"rotary: pairs are halves or neighbours, not {pairs!r}")
+    a.axes = axes
+    for i, n in enumerate(sections):
+        a.sections[i] = n
+    a.joint, a.neighbours, a.inverse, a.base = bool(joint), pairs == "neighbours", bool(inverse), base
+    _check(lib().hat_op_rotary(C.byref(a), stream), "rotary")
+
+
+def _sequences(cu, what):
+    if len(cu.shape) != 1 or cu.shape[0] < 1:
+        raise HatError(f"{what}: offsets of every sequence and the end of the last expected")
+    return cu.shape[0] - 1
+
+
+def _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k):
+    a = AttentionArgs()
+    a.dtype = code = _code(q, "attention: q")
+    a.q, bq, a.q_tokens, a.q_heads, a.head_dim = _heads(q, "attention: q", code)
+    a.k, bk, a.k_tokens, a.kv_heads, d = _heads(k, "attention: k", code)
+    a.v = _heads(v, "attention: v", code, tuple(k.shape))[0]
+    a.out = _heads(out, "attention: out", code, tuple(q.shape))[0]
+    if d != a.head_dim:
+        raise HatError(f"attention: head_dim {a.head_dim} of q and {d} of k")
+    n = _sequences(cu_q, "attention: cu_q") if cu_q is not None else None
+    if cu_k is not None:
+        m = _sequences(cu_k, "attention: cu_k")
+        if n is not None and m != n:
+            raise HatError(f"attention: {n} sequences in cu_q and {m} in cu_k")
+        n = m
+    if n is None:
+        n = bq
+    if (cu_q is not None and len(q.shape) != 3) or (cu_k is not None and len(k.shape) != 3):
+        raise HatError("attention: a packed tensor is [token, head, dim]")
+    if (cu_q is None and bq != n) or (cu_k is None and bk != n):
+        raise HatError(f"attention: q of {tuple(q.shape)} and k of {tuple(k.shape)} are not {n} sequences")
+    a.n_seq = n
+    a.cu_q = _vector(cu_q, "attention: cu_q", 3, n + 1)
+    a.cu_k = _vector(cu_k, "attention: cu_k", 3, n + 1)
+    a.q_lens = _vector(q_lens, "attention: q_lens", 3, n)
+    a.k_lens = _vector(k_lens, "attention: k_lens", 3, n)
+    a.prefix = _vector(prefix, "attention: prefix", 3, n)
+    a.slopes = _vector(slopes, "attention: slopes", 0, a.q_heads)
+    a.causal = bool(causal)
+    a.scale = a.head_dim ** -0.5 if scale is None else scale
+    a.cap = cap
+    if pos_q is not None and pos_k is not None:
+        a.pos_q, a.axes = _positions(pos_q, "attention: pos_q", bq, a.q_tokens)
+        a.pos_k, axes = _positions(pos_k, "attention: pos_k", bk, a.k_tokens)
+        if axes != a.axes:
+            raise HatError(f"attention: {a.axes} axes in pos_q and {axes} in pos_k")
+    elif pos_q is not None or pos_k is not None:
+        raise HatError("attention: positions of queries and keys go together")
+    return a
+
+
+def attention_workspace(q, k, v, out, scale=None, causal=False, prefix=None, cu_q=None, cu_k=None, q_lens=None,
+                        k_lens=None, cap=0.0, slopes=None, pos_q=None, pos_k=None):
+    """The bytes that op_attention of these arguments needs as its workspace."""
+    a = _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k)
+    n = lib().hat_op_attention_workspace(C.byref(a))
+    if n == C.c_size_t(-1).value:
+        raise HatError(f"attention: {_err()}")
+    return n
+
+
+def op_attention(q, k, v, out, scale=None, causal=False, prefix=None, cu_q=None, cu_k=None, q_lens=None, k_lens=None,
+                 cap=0.0, slopes=None, pos_q=None, pos_k=None, workspace=None, stream=None):
+    """hat_op_attention: [batch, token, head, dim] tensors, or packed [token, head, dim] with
+    cu_q / cu_k; scale None: head_dim^-1/2; workspace: a device tensor of at least
+    attention_workspace(...) bytes where that is not 0; stream as op_rotary's."""
+    a = _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k)
+    if workspace is not None:
+        size = _SIZES[_code(workspace, "attention: workspace")]
+        if len(workspace.shape) != 1 or (workspace.shape[0] > 1 and workspace.stride()[0] != 1):
+            raise HatError("attention: the workspace is one contiguous row")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.shape[0] * size
+    _check(lib().hat_op_attention(C.byref(a), stream), "attention")
+
+
+def _rows(t, what, code, lead=None):
+    if _code(t, what) != code:
+        raise HatError(f"{what}: type {t.dtype} differs from x's")
+    shape, st = tuple(t.shape), t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and st[1] != 1) or (lead is not None and shape != lead):
+        raise HatError(f"{what}: {shape} is no [rows, width] of stride 1" + (f" like x's {lead}" if lead else ""))
+    return t.data_ptr(), st[0]
+
+
+def op_residual_norm(x, y=None, x_out=None, h=None, gate=None, scale=1.0, post="none", post_weight=None,
+                     post_bias=None, pre="none", pre_weight=None, pre_bias=None, eps=1e-5, post_eps=None,
+                     stream=None):
+    """hat_op_residual_norm on [rows, width] tensors: x_out = x + scale * gate * N(y), h =
+    N(x_out), either left out where None. gate: [gates, width], a row for each rows / gates
+    rows; post, pre: "none", "layer" or "rms" with fp32 weights; post_eps None: eps."""
+    a = ResidualNormArgs()
+    a.dtype = code = _code(x, "residual_norm: x")
+    if code > 2:
+        raise HatError(f"residual_norm: type {x.dtype} is not supported")
+    a.x, a.x_stride = _rows(x, "residual_norm: x", code)
+    lead = tuple(x.shape)
+    a.rows, a.width = lead
+    if y is not None:
+        a.y, a.y_stride = _rows(y, "residual_norm: y", code, lead)
+    if x_out is not None:
+        a.x_out, a.x_out_stride = _rows(x_out, "residual_norm: x_out", code, lead)
+    if h is not None:
+        a.h, a.h_stride = _rows(h, "residual_norm: h", code, lead)
+    if gate is not None:
+        a.gate, a.gate_stride = _rows(gate, "residual_norm: gate", code)
+        n = gate.shape[0]
+        if gate.shape[1] != a.width or n < 1 or a.rows % n:
+            raise HatError(f"residual_norm: gates of {tuple(gate.shape)} for x of {lead}")
+        a.rows_per_gate = max(1, a.rows // n)
+    if post not in _NORMS or pre not in _NORMS:
+        raise HatError(f"residual_norm: norms are none, layer or rms, not {post!r}, {pre!r}")
+    a.post, a.pre = _NORMS[post], _NORMS[pre]
+    a.post_w = _vector(post_weight, "residual_norm: post_weight", 0, a.width)
+    a.post_b = _vector(post_bias, "residual_norm: post_bias", 0, a.width)
+    a.pre_w = _vector(pre_weight, "residual_norm: pre_weight", 0, a.width)
+    a.pre_b = _vector(pre_bias, "residual_norm: pre_bias", 0, a.width)
+    a.scale, a.pre_eps, a.post_eps = scale, eps, eps if post_eps is None else post_eps
+    _check(lib().hat_op_residual_norm(C.byref(a), stream), "residual_norm")

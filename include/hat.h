@@ -198,6 +198,109 @@ int hat_op_ocab(const float *x, float *out, int hp, int wp, int c, int heads, in
                 const float *n2b, const float *fc1_w, const float *fc1_b, const float *fc2_w,
                 const float *fc2_b, int iters, float *ms, float *attn_ms);
 
+/* ---- Operators on device tensors ------------------------------------------
+ *
+ * The transformer block around image and video tokens: rotary positions on
+ * several axes, attention over sequences, and the join with the residual stream
+ * (no reference counterpart; hat_op_swmsa and hat_op_ocab above are the
+ * network's own attention). Tensors are device memory of device 0 (from
+ * hat_device_alloc or another allocator of the process); strides count
+ * elements and the last axis always has stride 1. Types: HAT_F32, HAT_F16,
+ * HAT_BF16, one for all of a call's tensors; sums, softmax and norms are held
+ * in fp32 and every result is rounded once.
+ *
+ * A call checks its arguments, enqueues its kernels on `stream` (a hipStream_t
+ * of device 0; NULL: the default stream, as hat_device_copy) and returns; it
+ * neither allocates nor waits, so it can be captured into a graph. Outputs
+ * may be the inputs they replace (the same pointer and strides) where stated
+ * and must otherwise not overlap them. */
+enum { HAT_F32 = 0, HAT_F16 = 1, HAT_BF16 = 2 };
+
+/* [batch][token][head][dim] */
+typedef struct {
+    void *data;
+    long long batch_stride, token_stride, head_stride;
+} hat_heads;
+/* int32 [batch][token][axis]; batch_stride 0: one set for every batch entry. */
+typedef struct {
+    const int *data;
+    long long batch_stride, token_stride, axis_stride;
+} hat_positions;
+
+/* Rotary positions: pair i of axis a (0 <= i < sections[a]) of every head is
+ * turned by pos[token][a] * base^(-i / sections[a]), or, joint, by
+ * pos[token][a] * base^(-n / S) with n the pair's index over all axes and S
+ * their sum: (u, v) -> (u cos - v sin, v cos + u sin). Pair n is dims (n,
+ * n + S), or (2n, 2n + 1) with `neighbours`; dims from 2 S on are copied.
+ * inverse: by the negative angle, which is also the gradient. q and k are
+ * turned in one launch (k.data NULL: q alone); q_out, k_out may be q, k.
+ * head_dim <= 256. */
+typedef struct {
+    int dtype, batch, q_heads, k_heads, head_dim, axes;
+    long long tokens; /* of a batch entry */
+    int sections[4];
+    int joint, neighbours, inverse;
+    double base;
+    hat_positions pos;
+    hat_heads q, q_out, k, k_out;
+} hat_rotary;
+int hat_op_rotary(const hat_rotary *a, void *stream);
+
+/* Attention over n_seq sequences. Query head h reads key head
+ * h / (q_heads / kv_heads).
+ *   s(i, j) = c tanh(scale q_i . k_j / c) - slopes[h] * distance(i, j)
+ *   out_i   = sum_j e^s(i, j) v_j / sum_j e^s(i, j)
+ * over the keys that query i sees; zeros where it sees none (or where every
+ * weight is zero). cap 0: no tanh.
+ * distance: |i + Lk - Lq - j| in a sequence of Lq queries and Lk keys, or with
+ * positions the sum over the axes of |pos_q[i] - pos_k[j]| (differences below
+ * 2^31).
+ * Sequences: entry s of a batch, its first q_lens[s] queries and k_lens[s] keys
+ * (NULL: all q_tokens, k_tokens); or, with cu_q / cu_k (n_seq + 1 rising
+ * offsets), rows cu[s] .. cu[s + 1) of a packed tensor of q_tokens / k_tokens
+ * rows (its batch_stride is not used), which is the document mask. Lengths and
+ * offsets are int32 in device memory, clamped to the tensors. Rows of out that
+ * belong to no query keep what they hold.
+ * causal: query i sees keys j <= i + Lk - Lq, and keys below prefix[s] (NULL:
+ * none). Keys that a query does not see have no influence, whatever they hold.
+ * head_dim <= 128; out may be q. workspace: hat_op_attention_workspace bytes,
+ * 16-byte aligned, in use until the call's kernels end: calls (and captured
+ * graphs) that may run at the same time need one each. */
+typedef struct {
+    int dtype, n_seq, q_heads, kv_heads, head_dim, axes;
+    long long q_tokens, k_tokens;
+    hat_heads q, k, v, out;
+    const int *cu_q, *cu_k, *q_lens, *k_lens, *prefix;
+    int causal;
+    float scale, cap;
+    const float *slopes; /* [q_heads] in device memory, or NULL */
+    hat_positions pos_q, pos_k; /* data NULL: distance by index */
+    void *workspace;
+    size_t workspace_bytes;
+} hat_attention;
+/* Reads sizes only: pointers count as set or NULL. (size_t)-1 on error. */
+size_t hat_op_attention_workspace(const hat_attention *a);
+int hat_op_attention(const hat_attention *a, void *stream);
+
+/* The join with the residual stream and the norms before and after it, row by
+ * row of `width` values (<= 16384):
+ *   x' = x + scale * gate * Npost(y),   h = Npre(x')   (x' before its rounding)
+ * N: HAT_NORM_NONE, HAT_NORM_LAYER (v - mean) / sqrt(var + eps) * w + b, or
+ * HAT_NORM_RMS v / sqrt(mean v^2 + eps) * w + b; w, b fp32 [width] or NULL (ones,
+ * zeros). gate: rows of `width` values, one for each rows_per_gate rows (NULL:
+ * ones). y NULL: x' = x. x_out or h may be NULL; x_out and h may be x or y. */
+enum { HAT_NORM_NONE = 0, HAT_NORM_LAYER = 1, HAT_NORM_RMS = 2 };
+typedef struct {
+    int dtype, width, post, pre;
+    long long rows, rows_per_gate;
+    const void *x, *y, *gate;
+    void *x_out, *h;
+    long long x_stride, y_stride, gate_stride, x_out_stride, h_stride; /* of rows */
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    float scale, post_eps, pre_eps;
+} hat_residual_norm;
+int hat_op_residual_norm(const hat_residual_norm *a, void *stream);
+
 /* ---- Device memory and timing (lightgpu::vm DevBuf, src/cuda.rs:528-555) -- */
 void *hat_device_alloc(size_t bytes);
 int hat_device_free(void *p);
