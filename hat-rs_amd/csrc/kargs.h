@@ -401,8 +401,14 @@ struct SeqAttnArgs {
     int n_seq, q_heads, kv_heads, group, dim, axes;
     int q_tokens, k_tokens;  // of a batch entry, or of the packed tensor
     int causal;
+    int wide;                // q, k, v rows: 16-byte chunks (else element by element)
+    int wide_out;            // out rows: four elements at a time
     float scale;             // scores = scale * q . k
     float cap, inv_cap;      // cap > 0: cap * tanh(scores * inv_cap)
+    float c1;                // log2(e) scale, or 2 log2(e) scale / cap: what q . k is multiplied by
+    int tiles;               // tiles of rows a sequence (not packed), or in all
+    int chunk, slots;        // split form: keys a chunk; chunks a sequence (not packed), or in all
+    float *part, *part_ml;   // split form: a chunk's o [slot][kv_head][row][dim], and (m, l)
 };
 
 enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };

@@ -15,6 +15,24 @@ struct SeqView {
     long long bq, bk;         // batch index of the q and k tensors (0 where packed)
 };
 
+// Shapes. A stage of keys sits in LDS as rows of DP = 32 DT elements in 16-byte
+// chunks; chunk c of row r lies at slot c ^ swizzle(r), so that the reads down the
+// rows (K: 8 rows of one chunk at a time; 16-bit V: four rows of two chunks) meet
+// every bank once. fp32 V is read along its rows and needs none.
+template <class T, int DT>
+struct SeqShape {
+    static constexpr int DP = 32 * DT;
+    static constexpr int E = 16 / (int)sizeof(T);  // elements a chunk
+    static constexpr int CH = DP / E;              // chunks a row
+    static constexpr int KS = CH / 2;              // MFMA steps of q . k: two chunks each, one a lane half
+    static constexpr int ROW = DP * (int)sizeof(T);
+    __device__ static __forceinline__ int kswz(int r) { return CH % 8 ? (r >> 1) & 3 : r & 7; }
+    __device__ static __forceinline__ int vswz(int r)
+    {
+        return sizeof(T) == 4 ? 0 : CH % 8 ? (r & 2) : (r & 3) << 1;
+    }
+};
+
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Offsets and lengths come from device memory: clamped, so that no value of theirs
@@ -64,10 +82,13 @@ __device__ __forceinline__ float lane_value(float v, int lane)
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-// One row by one wave, in fp32 throughout, every product of its own: keys that the
-// row does not see are not touched, whatever they hold.
+// Keys [j0, j1) of one row by one wave, in fp32 throughout, every product of its own:
+// keys that the row does not see are not touched, whatever they hold. m: the largest
+// score (log2 units), l: the sum of 2^(s - m), oa, oc: dims lane and lane + 64 of the
+// sum of 2^(s - m) v.
 template <class T>
-__device__ void attn_row(const SeqAttnArgs& p, const SeqView& v, int i, int head, int limit)
+__device__ void attn_row(const SeqAttnArgs& p, const SeqView& v, int i, int head, int j0, int j1, float& m, float& l,
+                         float& oa, float& oc)
 {
     const int lane = threadIdx.x & 63;
     const int D = p.dim, kvh = head / p.group;
@@ -76,12 +97,12 @@ __device__ void attn_row(const SeqAttnArgs& p, const SeqView& v, int i, int head
     const T* vv = (const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + kvh * p.vh;
     const float qa = lane < D ? (float)q[lane] : 0.0f, qc = lane + 64 < D ? (float)q[lane + 64] : 0.0f;
     const float slope = p.slopes ? p.slopes[head] * HAT_LOG2E : 0.0f;
-    float m = -INFINITY, l = 0.0f, oa = 0.0f, oc = 0.0f;
-    for (int j0 = 0; j0 < limit; j0 += 64) {
+    m = -INFINITY, l = oa = oc = 0.0f;
+    for (; j0 < j1; j0 += 64) {
         const int j = j0 + lane;
-        // every lane takes part, those past the limit on the last key: a lane's value
+        // every lane takes part, those past the end on the last key: a lane's value
         // is read by all (v_readlane), so it must be computed by all
-        const int jr = j < limit ? j : limit - 1;
+        const int jr = j < j1 ? j : j1 - 1;
         const T* kr = k + (long long)jr * p.kt;
         float s = 0.0f;
         for (int d = 0; d < D && d < 64; ++d) s = __builtin_fmaf(lane_value(qa, d), (float)kr[d], s);
@@ -101,15 +122,15 @@ __device__ void attn_row(const SeqAttnArgs& p, const SeqView& v, int i, int head
             }
             s = __builtin_fmaf(-slope, far, s);
         }
-        s = j < limit ? s : -INFINITY;
+        s = j < j1 ? s : -INFINITY;
         const float mn = fmaxf(m, wave_max(s));
         const float base = mn == -INFINITY ? 0.0f : mn;
-        const float e = j < limit ? fast_exp2(s - base) : 0.0f;
+        const float e = j < j1 ? fast_exp2(s - base) : 0.0f;
         const float corr = fast_exp2(m - base);
         l = l * corr + wave_sum(e);
         oa *= corr;
         oc *= corr;
-        const int n = limit - j0 < 64 ? limit - j0 : 64;
+        const int n = j1 - j0 < 64 ? j1 - j0 : 64;
         for (int t = 0; t < n; ++t) {
             const float pt = lane_value(e, t);
             const T* vr = vv + (long long)(j0 + t) * p.vt;
@@ -118,46 +139,777 @@ __device__ void attn_row(const SeqAttnArgs& p, const SeqView& v, int i, int head
         }
         m = mn;
     }
-    T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + i) * p.ot + head * p.oh;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (lane < D) o[lane] = (T)(oa * inv);
-    if (lane + 64 < D) o[lane + 64] = (T)(oc * inv);
 }
 
-// A wave a row, four rows a block.
-template <class T>
-__device__ __forceinline__ void attn_rows_body(const SeqAttnArgs& p)
+__device__ __forceinline__ float join_scale(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+__device__ __forceinline__ float swap_max(float v)  // over a lane and its twin in the other half
 {
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int head = (int)(row % p.q_heads);
-    const long long tok = row / p.q_heads;
-    int s, i;
-    if (p.cu_q) {
-        if (tok >= p.q_tokens) return;
-        int lo = 0, hi = p.n_seq;  // the first sequence that ends behind the token
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (p.cu_q[mid + 1] > tok)
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        s = lo;
-        if (s == p.n_seq) return;
-        i = (int)tok - clamp_int(p.cu_q[s], 0, p.q_tokens);
-    } else {
-        s = (int)(tok / p.q_tokens);
-        i = (int)(tok - (long long)s * p.q_tokens);
-        if (s >= p.n_seq) return;
-    }
-    const SeqView v = seq_view(p, s);
-    if (i < 0 || i >= v.lq) return;
-    attn_row<T>(p, v, i, head, row_limit(p, v, i, p.prefix ? p.prefix[s] : 0));
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const unsigned b = __float_as_uint(v);
+    const u2 r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-#define SEQ_ROWS_INST(NAME, T) \
-    extern "C" __global__ __launch_bounds__(256) void NAME(SeqAttnArgs p) { attn_rows_body<T>(p); }
+__device__ __forceinline__ float swap_sum(float v)
+{
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const unsigned b = __float_as_uint(v);
+    const u2 r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
-SEQ_ROWS_INST(hat_attnseq_rows_f32, float)
-SEQ_ROWS_INST(hat_attnseq_rows_f16, f16)
-SEQ_ROWS_INST(hat_attnseq_rows_bf16, bf16)
+__device__ __forceinline__ f32x16 mma16(u32x4 a, u32x4 b, f32x16 c, f16) { return mfma_f16(a, b, c); }
+__device__ __forceinline__ f32x16 mma16(u32x4 a, u32x4 b, f32x16 c, bf16)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ unsigned pack16(float a, float b, f16)
+{
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, f16x2));
+}
+__device__ __forceinline__ unsigned pack16(float a, float b, bf16) { return pk_bf16(a, b); }
+
+// The rows of K or V of one stage into LDS, by THREADS threads (a block, or one wave on
+// its own): R rows from row `first` of n, zeros past the last and past the head's dims.
+// Chunks go straight to LDS through a buffer descriptor that ends with the last row,
+// whose range check supplies the zeros without a branch.
+template <class T, int DT, int R, int THREADS, bool V>
+struct Stage {
+    using S = SeqShape<T, DT>;
+    static constexpr int N = R * S::CH / THREADS;
+    static_assert(R * S::CH % THREADS == 0, "whole moves a thread");
+    const T* base;     // the sequence's first row, this head
+    long long stride;  // of rows
+    int n, dim;
+    unsigned off[N];   // the lane's byte offset from the stage's first row, per move
+    __device__ __forceinline__ void init(const T* b, long long st, int rows, int d, int tid)
+    {
+        base = b, stride = st, n = rows, dim = d;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = j * THREADS + tid, r = c / S::CH, lc = (c % S::CH) ^ (V ? S::vswz(r) : S::kswz(r));
+            off[j] = lc * S::E < dim ? (unsigned)(r * (int)stride * (int)sizeof(T) + lc * 16) : 0x80000000u;
+        }
+    }
+    __device__ __forceinline__ void issue(unsigned char* lds, int first, int tid, int wide) const
+    {
+        const int left = n - first;
+        const T* b = base + (long long)first * stride;
+        if (wide) {
+            const int rows = left < R ? left : R;
+            const int bytes = rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * (int)sizeof(T);
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, bytes, 0x00027000);
+            unsigned char* to = lds + (THREADS > 64 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0) * 1024;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rsrc, (__attribute__((address_space(3))) void*)(to + j * THREADS * 16), 16, off[j], 0, 0, 0);
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < N; ++j) {
+                const int c = j * THREADS + tid, r = c / S::CH, d0 = ((c % S::CH) ^ (V ? S::vswz(r) : S::kswz(r))) * S::E;
+                typename Vec<T, S::E>::type u;
+#pragma unroll
+                for (int e = 0; e < S::E; ++e) u[e] = r < left && d0 + e < dim ? b[(long long)r * stride + d0 + e] : (T)0.0f;
+                *(decltype(u)*)(lds + c * 16) = u;
+            }
+        }
+    }
+};
+
+// What a lane knows of its row: row r of a (sequence, key head) pair is query r / group,
+// head r % group of the pair's heads.
+struct SeqRow {
+    int i, head;
+    bool live;
+};
+
+__device__ __forceinline__ SeqRow seq_row(const SeqAttnArgs& p, int r, int rows, int kvh)
+{
+    const int i = r / p.group;
+    return {i, kvh * p.group + r - i * p.group, r < rows};
+}
+
+// The lane's q as the B operand of K Q^T: step ks holds the lane half's chunk 2 ks + h.
+template <class T, int DT>
+__device__ __forceinline__ void load_q(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r,
+                                       u32x4 (&q)[SeqShape<T, DT>::KS])
+{
+    using S = SeqShape<T, DT>;
+    const int h = (threadIdx.x >> 5) & 1;
+    const T* row = (const T*)p.q + v.bq * p.qb + (long long)(v.q0 + r.i) * p.qt + r.head * p.qh;
+    const bool flip = p.scale < 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+        const int d0 = (2 * ks + h) * S::E;
+        u32x4 u = {0, 0, 0, 0};
+        if (r.live && d0 < p.dim) {
+            if (p.wide) {
+                u = *(const u32x4*)(row + d0);
+            } else {
+                typename Vec<T, S::E>::type w;
+#pragma unroll
+                for (int e = 0; e < S::E; ++e) w[e] = d0 + e < p.dim ? row[d0 + e] : (T)0.0f;
+                u = __builtin_bit_cast(u32x4, w);
+            }
+        }
+        if (flip) {  // c1 is positive
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+        }
+        q[ks] = u;
+    }
+}
+
+// One lane's running softmax over the keys of its row.
+template <class T, int DT>
+struct SeqAcc {
+    f32x16 o[DT];
+    float m, l;
+    __device__ __forceinline__ void init()
+    {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+        m = -1e30f, l = 0.0f;  // finite: 2^(-inf - m) is 0, not NaN
+    }
+};
+
+// The bias of a lane's row.
+struct SeqBias {
+    float slope;      // log2 units
+    int at;           // i + Lk - Lq
+    unsigned pos[4];  // positions, offset to order as unsigned
+};
+
+template <class T>
+__device__ __forceinline__ SeqBias seq_bias(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r)
+{
+    SeqBias b;
+    b.slope = p.slopes && r.live ? p.slopes[r.head] * HAT_LOG2E : 0.0f;
+    b.at = r.i + v.lk - v.lq;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        b.pos[a] = 0;
+        if (p.pos_q && r.live && a < p.axes)
+            b.pos[a] = (unsigned)p.pos_q[v.bq * p.pqb + (long long)(v.q0 + r.i) * p.pqt + a * p.pqa] ^ 0x80000000u;
+    }
+    return b;
+}
+
+// The scores of 32 keys from k0 in log2 units: the cap and the bias on q . k. pk: the
+// keys' positions in LDS, one row of `pstride` an axis. Register r is key
+// 8 (r / 4) + 4 h + r % 4.
+template <class T>
+__device__ __forceinline__ void seq_scores(const SeqAttnArgs& p, const SeqBias& b, f32x16& s, int k0, const unsigned* pk,
+                                           int pstride)
+{
+    const int h = (threadIdx.x >> 5) & 1;
+    if (p.cap > 0.0f) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = p.cap * HAT_LOG2E * tanhf(s[r] * fabsf(p.scale) * p.inv_cap);
+        } else {
+            // tanh x = 1 - 2 / (e^2x + 1): off by 2^-23 of the cap, which the
+            // probabilities' rounding to 16 bits covers
+            const float a = p.cap * HAT_LOG2E;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[r] = __builtin_fmaf(-2.0f * a, __builtin_amdgcn_rcpf(fast_exp2(s[r] * p.c1) + 1.0f), a);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= p.c1;
+    }
+    if (!p.slopes) return;
+    if (!p.pos_q) {
+        const float at = (float)(b.at - k0 - 4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-b.slope, fabsf(at - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+    } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            unsigned far[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                if (a < p.axes) {
+                    const u32x4 k = *(const u32x4*)(pk + a * pstride + 8 * g + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) far[e] += max(b.pos[a], k[e]) - min(b.pos[a], k[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_fmaf(-b.slope, (float)far[e], s[4 * g + e]);
+        }
+    }
+}
+
+// One stage of KT x 32 keys for QT x 32 rows of a wave: S^T = K Q^T (A = 32 keys, B =
+// the wave's q), so that a lane holds 16 scores of one row and, as probabilities, the B
+// operand of O^T += V^T P^T without a move. With MFMA's key order within 16 (lane half h,
+// slot j: keys 4 h + j, then 8 + 4 h + j - 4) V's operand is two transposed reads of
+// four keys each. The running maximum moves only when a score passes it by 2^8, so the
+// sums are seldom rescaled; P stays below 2^8.
+template <class T, int DT, int QT, int KT, bool GEN>
+__device__ __forceinline__ void seq_stage(const SeqAttnArgs& p, const unsigned char* K, const unsigned char* V,
+                                          const unsigned* pk, int pstride, const u32x4 (&q)[QT][SeqShape<T, DT>::KS],
+                                          SeqAcc<T, DT> (&acc)[QT], const SeqBias (&bias)[QT], const int (&limit)[QT],
+                                          int k0, bool masked)
+{
+    using S = SeqShape<T, DT>;
+    const int lane = threadIdx.x & 63, ql = lane & 31, h = lane >> 5;
+    f32x16 s[QT][KT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][kt][r] = 0.0f;
+    const int krow = ql * S::ROW, ksw = S::kswz(ql);
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+        const int at = krow + (((2 * ks + h) ^ ksw) << 4);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            const u32x4 a = *(const u32x4*)(K + at + kt * 32 * S::ROW);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t][kt] = mfma32(__uint_as_float(a[e]), __uint_as_float(q[t][ks][e]), s[t][kt]);
+                } else {
+                    s[t][kt] = mma16(a, q[t][ks], s[t][kt], T());
+                }
+            }
+        }
+    }
+    u32x4 pb[QT][KT][2];  // 16-bit types: P packed, 16 keys each
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        SeqAcc<T, DT>& c = acc[t];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            if constexpr (GEN) seq_scores<T>(p, bias[t], s[t][kt], k0 + 32 * kt, pk + 32 * kt, pstride);
+            if (masked) {
+                const int left = limit[t] - k0 - 32 * kt - 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][kt][r] = 8 * (r >> 2) + (r & 3) < left ? s[t][kt][r] : -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][kt][r]);
+        }
+        mx = swap_max(mx);
+        if constexpr (!GEN) mx *= p.c1;
+        if (__any(mx > c.m + 8.0f)) {
+            const float mn = fmaxf(c.m, mx), corr = fast_exp2(c.m - mn);
+            c.m = mn;
+            c.l *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) c.o[d][r] *= corr;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = fast_exp2(GEN ? s[t][kt][r] - c.m : __builtin_fmaf(s[t][kt][r], p.c1, -c.m));
+                s[t][kt][r] = e;
+                c.l += e;
+            }
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) pb[t][kt][r >> 3][(r & 7) >> 1] = pack16(s[t][kt][r], s[t][kt][r + 1], T());
+            }
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const unsigned char* row = V + (32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)) * S::ROW + ql * 4;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const float a = *(const float*)(row + d * 128);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) acc[t].o[d] = mfma32(a, s[t][kt][r], acc[t].o[d]);
+                }
+            }
+    } else {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const int x = lane & 15, kr = 4 * h + (x >> 2);
+        const int row = kr * S::ROW + (x & 1) * 8;
+        const int lc = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1), vsw = S::vswz(kr);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const unsigned char* at = V + row + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4*)(at + 8 * S::ROW));
+                    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+                    const u2 a = __builtin_bit_cast(u2, lo), b = __builtin_bit_cast(u2, hi);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        acc[t].o[d] = mma16((u32x4){a[0], a[1], b[0], b[1]}, pb[t][kt][st], acc[t].o[d], T());
+                }
+    }
+}
+
+// Whether a lane's row came out finite (l and every o).
+template <class T, int DT>
+__device__ __forceinline__ bool seq_finite(const SeqAcc<T, DT>& c)
+{
+    float z = c.l * 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(c.o[d][r], 0.0f, z);
+    return z == 0.0f;
+}
+
+// The sequence of slot `at` where sequence s owns the slots from cu[s] * mul / per + s
+// on: enough for ceil(length * mul / per) each, whatever the lengths, so the host needs
+// only the totals. All lanes look at 64 sequences at a time; -1: none.
+__device__ __forceinline__ int find_sequence(const int* cu, int n, int total, int mul, int per, int at, int& first)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n;  // the last s with slot(s) <= at lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64;
+        const int s = lo + lane * step;
+        bool ok = false;
+        if (s < hi) ok = (long long)clamp_int(cu[s], 0, total) * mul / per + s <= at;
+        const int c = __popcll(__ballot(ok));
+        if (c == 0) return -1;
+        lo += (c - 1) * step;
+        if (lo + step < hi) hi = lo + step;
+    }
+    first = (int)((long long)clamp_int(cu[lo], 0, total) * mul / per) + lo;
+    return first <= at ? lo : -1;
+}
+
+__device__ __forceinline__ SeqView uniform(const SeqView& v)
+{
+    SeqView w;
+    w.s = __builtin_amdgcn_readfirstlane(v.s);
+    w.lq = __builtin_amdgcn_readfirstlane(v.lq);
+    w.lk = __builtin_amdgcn_readfirstlane(v.lk);
+    w.q0 = __builtin_amdgcn_readfirstlane(v.q0);
+    w.k0 = __builtin_amdgcn_readfirstlane(v.k0);
+    w.bq = v.bq ? w.s : 0;
+    w.bk = v.bk ? w.s : 0;
+    return w;
+}
+
+// ---- many rows: a block of four waves, QT x 32 rows each, walks the keys in stages of
+// KT x 32, two in LDS: the next one's copy runs under the present one's products.
+template <class T, int DT, int QT, int KT, bool GEN>
+__device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0, unsigned char* K1, unsigned char* V0,
+                                         unsigned char* V1, unsigned* P0, unsigned* P1)
+{
+    constexpr int BQ = 128 * QT, BK = 32 * KT;
+    const int pairs = p.cu_q ? p.kv_heads : p.kv_heads * p.n_seq;
+    const int pair = blockIdx.x % pairs;
+    int tile = blockIdx.x / pairs, sq, kvh;
+    if (p.cu_q) {
+        int first = 0;
+        kvh = pair;
+        sq = find_sequence(p.cu_q, p.n_seq, p.q_tokens, p.group, BQ, tile, first);
+        if (sq < 0) return;
+        tile -= first;
+    } else {
+        sq = pair / p.kv_heads;
+        kvh = pair - sq * p.kv_heads;
+    }
+    const SeqView v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    const int rows = v.lq * p.group;
+    const int tiles = (rows + BQ - 1) / BQ;
+    if (tile >= tiles) return;
+    if (p.causal) tile = tiles - 1 - tile;  // the longest first
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
+    const int row0 = tile * BQ + wave * 32 * QT;
+    const int row_last = tile * BQ + BQ - 1 < rows ? tile * BQ + BQ - 1 : rows - 1;
+    const int end = row_limit(p, v, row_last / p.group, prefix);
+
+    u32x4 q[QT][SeqShape<T, DT>::KS];
+    SeqAcc<T, DT> acc[QT];
+    SeqBias bias[QT];
+    SeqRow row[QT];
+    int limit[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        row[t] = seq_row(p, row0 + 32 * t + (lane & 31), rows, kvh);
+        load_q<T, DT>(p, v, row[t], q[t]);
+        limit[t] = row[t].live ? row_limit(p, v, row[t].i, prefix) : 0x7fffffff;
+        if constexpr (GEN) bias[t] = seq_bias<T>(p, v, row[t]);
+        acc[t].init();
+    }
+    // limits rise with the row: the wave's least and largest
+    int least = 0x7fffffff, most = 0;
+    if (row0 < rows) {
+        least = row_limit(p, v, row0 / p.group, prefix);
+        const int last = row0 + 32 * QT - 1 < rows ? row0 + 32 * QT - 1 : rows - 1;
+        most = row_limit(p, v, last / p.group, prefix);
+    }
+
+    Stage<T, DT, BK, 256, false> sk;
+    Stage<T, DT, BK, 256, true> sv;
+    sk.init((const T*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + kvh * p.kh, p.kt, v.lk, p.dim, tid);
+    sv.init((const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + kvh * p.vh, p.vt, v.lk, p.dim, tid);
+    const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
+    const auto issue = [&](unsigned char* K, unsigned char* V, unsigned* P, int k0) {
+        sk.issue(K, k0, tid, p.wide);
+        sv.issue(V, k0, tid, p.wide);
+        if constexpr (GEN) {
+            if (p.pos_q)
+                for (int e = tid; e < p.axes * BK; e += 256) {
+                    const int a = e / BK, j = k0 + e % BK;
+                    P[e] = j < v.lk ? (unsigned)pos_k[(long long)j * p.pkt + a * p.pka] ^ 0x80000000u : 0u;
+                }
+        }
+    };
+    const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
+        if (k0 < most) seq_stage<T, DT, QT, KT, GEN>(p, K, V, P, BK, q, acc, bias, limit, k0, k0 + BK > least);
+    };
+    if (end > 0) {
+        issue(K0, V0, P0, 0);
+        __syncthreads();
+        for (int k0 = 0; k0 < end; k0 += 2 * BK) {
+            issue(K1, V1, P1, k0 + BK);  // past the last key: zeros
+            stage(K0, V0, P0, k0);
+            __syncthreads();
+            if (k0 + BK >= end) break;
+            issue(K0, V0, P0, k0 + 2 * BK);
+            stage(K1, V1, P1, k0 + BK);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        SeqAcc<T, DT>& c = acc[t];
+        c.l = swap_sum(c.l);
+        // A probability of 0 does not keep out a NaN or an infinity of an unseen key in
+        // a tile that holds seen ones: such rows are done again, key by key.
+        const bool bad = row[t].live && !seq_finite(c);
+        T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + row[t].i) * p.ot + row[t].head * p.oh;
+        const unsigned long long all = __ballot(bad);
+        unsigned redo = (unsigned)(all | all >> 32);
+        const bool mine = (redo >> (lane & 31)) & 1;
+        if (row[t].live && !mine) {
+            const float inv = join_scale(c.l);
+            const int h = lane >> 5;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int at = 32 * d + 8 * g + 4 * h;
+                    float f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = c.o[d][4 * g + e] * inv;
+                    if (p.wide_out) {
+                        if (at < p.dim) store_vec<T, 4>(o + at, f);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (at + e < p.dim) o[at + e] = (T)f[e];
+                    }
+                }
+        }
+        while (redo) {
+            const int x = __builtin_ctz(redo);
+            redo &= redo - 1;
+            const SeqRow r = seq_row(p, row0 + 32 * t + x, rows, kvh);
+            float m, l, oa, oc;
+            attn_row<T>(p, v, r.i, r.head, 0, row_limit(p, v, r.i, prefix), m, l, oa, oc);
+            T* ro = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + r.i) * p.ot + r.head * p.oh;
+            if (lane < p.dim) ro[lane] = (T)(oa * join_scale(l));
+            if (lane + 64 < p.dim) ro[lane + 64] = (T)(oc * join_scale(l));
+        }
+    }
+}
+
+// ---- few rows a sequence (a token each, say) against many keys: the keys go over blocks
+// in chunks and over a block's W waves in tiles of 32, each wave with LDS and a pipeline of
+// its own; the waves' sums are joined in LDS, the chunks' by hat_attnseq_join.
+template <class T, int DT, int W>
+struct SplitShape {
+    static constexpr int TILE = 32 * SeqShape<T, DT>::ROW;  // a wave's stage of K or V
+    static constexpr int XROW = 36;                         // floats of a joined row's 32 dims
+    static constexpr int BYTES = W * TILE > W * 32 * XROW * 4 ? W * TILE : W * 32 * XROW * 4;
+};
+
+// Partial results of a (chunk slot, key head): rows of dim values, rows of (m, l).
+__device__ __forceinline__ long long part_row(const SeqAttnArgs& p, int slot, int kvh, int r)
+{
+    return ((long long)slot * p.kv_heads + kvh) * ((long long)p.q_tokens * p.group) + r;
+}
+
+template <class T, int DT, int W>
+__device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned char* B0, unsigned char* B1,
+                                               unsigned char* B2, unsigned char* B3, unsigned* P0, unsigned* P1,
+                                               float* ml, unsigned* flags)
+{
+    using X = SplitShape<T, DT, W>;
+    constexpr int DP = 32 * DT;
+    // b = (slot * kv_heads + kvh) * tiles + tile
+    const int tile = blockIdx.x % p.tiles;
+    const int kvh = blockIdx.x / p.tiles % p.kv_heads;
+    const int slot = blockIdx.x / p.tiles / p.kv_heads;
+    int sq, chunk;
+    if (p.cu_k) {
+        int first = 0;
+        sq = find_sequence(p.cu_k, p.n_seq, p.k_tokens, 1, p.chunk, slot, first);
+        if (sq < 0) return;
+        chunk = slot - first;
+    } else {
+        sq = slot / p.slots;
+        chunk = slot - sq * p.slots;
+    }
+    const SeqView v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    const int rows = v.lq * p.group;
+    const int row0 = tile * 32;
+    if (row0 >= rows) return;
+    const int prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
+    const int last = row0 + 31 < rows ? row0 + 31 : rows - 1;
+    const int least = row_limit(p, v, row0 / p.group, prefix), end = row_limit(p, v, last / p.group, prefix);
+    const int c0 = chunk * p.chunk;
+    if (c0 >= end && chunk > 0) return;  // no row's join asks for it; chunk 0 writes the empty rows
+    const int c1 = end - c0 < p.chunk ? end : c0 + p.chunk;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    u32x4 q[1][SeqShape<T, DT>::KS];
+    SeqAcc<T, DT> acc[1];
+    SeqBias bias[1];
+    int limit[1];
+    const SeqRow row = seq_row(p, row0 + (lane & 31), rows, kvh);
+    load_q<T, DT>(p, v, row, q[0]);
+    limit[0] = row.live ? row_limit(p, v, row.i, prefix) : 0x7fffffff;
+    bias[0] = seq_bias<T>(p, v, row);
+    acc[0].init();
+
+    Stage<T, DT, 32, 64, false> sk;
+    Stage<T, DT, 32, 64, true> sv;
+    sk.init((const T*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + kvh * p.kh, p.kt, c1, p.dim, lane);
+    sv.init((const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + kvh * p.vh, p.vt, c1, p.dim, lane);
+    const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
+    const int lds = wave * X::TILE;
+    constexpr int MOVES = 2 * Stage<T, DT, 32, 64, false>::N;
+    const auto issue = [&](unsigned char* K, unsigned char* V, unsigned* P, int k0) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer's reads are done
+        sk.issue(K + lds, k0, lane, p.wide);
+        sv.issue(V + lds, k0, lane, p.wide);
+        if (p.pos_q)
+            for (int e = lane; e < p.axes * 32; e += 64) {
+                const int a = e >> 5, j = k0 + (e & 31);
+                P[wave * 128 + e] = j < c1 ? (unsigned)pos_k[(long long)j * p.pkt + a * p.pka] ^ 0x80000000u : 0u;
+            }
+    };
+    const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
+        // the other buffer's moves may still be under way
+        if (p.wide) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOVES) : "memory");
+        // limits end the chunk as well: keys behind it lie in another
+        seq_stage<T, DT, 1, 1, true>(p, K + lds, V + lds, P + wave * 128, 32, q, acc, bias, limit, k0,
+                                     k0 + 32 > least || k0 + 32 > c1);
+    };
+    limit[0] = limit[0] < c1 ? limit[0] : c1;
+    int k0 = c0 + 32 * wave;
+    issue(B0, B2, P0, k0);
+    while (k0 < c1) {
+        issue(B1, B3, P1, k0 + 32 * W);
+        stage(B0, B2, P0, k0);
+        k0 += 32 * W;
+        if (k0 >= c1) break;
+        issue(B0, B2, P0, k0 + 32 * W);
+        stage(B1, B3, P1, k0);
+        k0 += 32 * W;
+    }
+
+    // the waves' sums side by side: 32 dims of each row in a buffer
+    SeqAcc<T, DT>& c = acc[0];
+    c.l = swap_sum(c.l);
+    if (tid == 0) *flags = 0;
+    __syncthreads();  // every wave is through its stages, and its moves have arrived
+    const int h = lane >> 5, ql = lane & 31;
+    unsigned char* buf[4] = {B0, B1, B2, B3};
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(f32x4*)((float*)buf[d] + (wave * 32 + ql) * X::XROW + 8 * g + 4 * h) =
+                (f32x4){c.o[d][4 * g], c.o[d][4 * g + 1], c.o[d][4 * g + 2], c.o[d][4 * g + 3]};
+    if (h == 0) ml[(wave * 32 + ql) * 2] = c.m, ml[(wave * 32 + ql) * 2 + 1] = c.l;
+    __syncthreads();
+    constexpr int N = 32 * DP / (64 * W);  // values a thread: one dim of every (64 W / 32)th row
+    const int x = tid & 31;
+    float o[N], m[N / DT], l[N / DT];
+#pragma unroll
+    for (int n = 0; n < N / DT; ++n) {
+        const int r = (tid >> 5) + n * 2 * W;
+        m[n] = ml[r * 2];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m[n] = fmaxf(m[n], ml[(w * 32 + r) * 2]);
+        l[n] = 0.0f;
+        float f[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            f[w] = fast_exp2(ml[(w * 32 + r) * 2] - m[n]);
+            l[n] += f[w] * ml[(w * 32 + r) * 2 + 1];
+        }
+        float z = l[n] * 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) sum = __builtin_fmaf(f[w], ((const float*)buf[d])[(w * 32 + r) * X::XROW + x], sum);
+            o[n * DT + d] = sum;
+            z = __builtin_fmaf(sum, 0.0f, z);
+        }
+        if (row0 + r < rows && !(z == 0.0f)) atomicOr(flags, 1u << r);
+    }
+    __syncthreads();
+    const unsigned bad = *flags;  // rows to do again key by key, as in seq_body
+    const bool whole = p.part == nullptr;
+#pragma unroll
+    for (int n = 0; n < N / DT; ++n) {
+        const int r = (tid >> 5) + n * 2 * W;
+        if (row0 + r >= rows || ((bad >> r) & 1)) continue;
+        const SeqRow sr = seq_row(p, row0 + r, rows, kvh);
+        T* out = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + sr.i) * p.ot + sr.head * p.oh;
+        const long long pr = part_row(p, slot, kvh, row0 + r);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int at = 32 * d + x;
+            if (at < p.dim) {
+                if (whole)
+                    out[at] = (T)(o[n * DT + d] * join_scale(l[n]));
+                else
+                    p.part[pr * p.dim + at] = o[n * DT + d];
+            }
+        }
+        if (!whole && x == 0) p.part_ml[2 * pr] = m[n], p.part_ml[2 * pr + 1] = l[n];
+    }
+    for (int r = wave; r < 32; r += W) {
+        if (!((bad >> r) & 1)) continue;
+        const SeqRow sr = seq_row(p, row0 + r, rows, kvh);
+        int to = row_limit(p, v, sr.i, prefix);
+        to = to < c1 ? to : c1;
+        float rm, rl, oa, oc;
+        attn_row<T>(p, v, sr.i, sr.head, c0, to, rm, rl, oa, oc);
+        T* out = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + sr.i) * p.ot + sr.head * p.oh;
+        const long long pr = part_row(p, slot, kvh, row0 + r);
+        if (whole) {
+            if (lane < p.dim) out[lane] = (T)(oa * join_scale(rl));
+            if (lane + 64 < p.dim) out[lane + 64] = (T)(oc * join_scale(rl));
+        } else {
+            if (lane < p.dim) p.part[pr * p.dim + lane] = oa;
+            if (lane + 64 < p.dim) p.part[pr * p.dim + lane + 64] = oc;
+            if (lane == 0) p.part_ml[2 * pr] = rm == -INFINITY ? -1e30f : rm, p.part_ml[2 * pr + 1] = rl;
+        }
+    }
+}
+
+// The join of a row's chunks, a wave a row: o = sum 2^(m_c - m) o_c / sum 2^(m_c - m) l_c.
+template <class T>
+__device__ __forceinline__ void seq_join_body(const SeqAttnArgs& p)
+{
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long per = (long long)p.q_tokens * p.group;
+    const long long pair = at / per;
+    const int r = (int)(at - pair * per), lane = threadIdx.x & 63;
+    const int sq = (int)(pair / p.kv_heads), kvh = (int)(pair - (long long)sq * p.kv_heads);
+    if (sq >= p.n_seq) return;
+    const SeqView v = seq_view(p, sq);
+    if (r >= v.lq * p.group) return;
+    const SeqRow row = seq_row(p, r, v.lq * p.group, kvh);
+    const int limit = row_limit(p, v, row.i, p.prefix ? p.prefix[sq] : 0);
+    const int n = (int)(((long long)limit + p.chunk - 1) / p.chunk);
+    const int slot = p.cu_k ? v.k0 / p.chunk + sq : sq * p.slots;
+    float m = -1e30f;
+    for (int c = lane; c < n; c += 64) m = fmaxf(m, p.part_ml[2 * part_row(p, slot + c, kvh, r)]);
+    m = wave_max(m);
+    float l = 0.0f, oa = 0.0f, oc = 0.0f;
+    for (int c = 0; c < n; ++c) {
+        const long long pr = part_row(p, slot + c, kvh, r);
+        const float f = fast_exp2(p.part_ml[2 * pr] - m);
+        l = __builtin_fmaf(f, p.part_ml[2 * pr + 1], l);
+        if (lane < p.dim) oa = __builtin_fmaf(f, p.part[pr * p.dim + lane], oa);
+        if (lane + 64 < p.dim) oc = __builtin_fmaf(f, p.part[pr * p.dim + lane + 64], oc);
+    }
+    T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + row.i) * p.ot + row.head * p.oh;
+    if (lane < p.dim) o[lane] = (T)(oa * join_scale(l));
+    if (lane + 64 < p.dim) o[lane + 64] = (T)(oc * join_scale(l));
+}
+
+#define SEQ_INST(NAME, T, DT, QT, KT, GEN, WPS)                                                              \
+    extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
+    {                                                                                                        \
+        constexpr int B = 32 * KT * SeqShape<T, DT>::ROW;                                                    \
+        __shared__ __attribute__((aligned(16))) unsigned char K0[B], K1[B], V0[B], V1[B];                    \
+        __shared__ __attribute__((aligned(16))) unsigned P0[GEN ? 128 * KT : 4], P1[GEN ? 128 * KT : 4];     \
+        seq_body<T, DT, QT, KT, GEN>(p, K0, K1, V0, V1, P0, P1);                                             \
+    }
+
+SEQ_INST(hat_attnseq_f16_d1, f16, 1, 2, 2, false, 2)
+SEQ_INST(hat_attnseq_f16_d2, f16, 2, 2, 2, false, 2)
+SEQ_INST(hat_attnseq_f16_d3, f16, 3, 1, 2, false, 2)
+SEQ_INST(hat_attnseq_f16_d4, f16, 4, 1, 2, false, 2)
+SEQ_INST(hat_attnseq_f16_d1_gen, f16, 1, 2, 2, true, 2)
+SEQ_INST(hat_attnseq_f16_d2_gen, f16, 2, 2, 2, true, 2)
+SEQ_INST(hat_attnseq_f16_d3_gen, f16, 3, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_f16_d4_gen, f16, 4, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_bf16_d1, bf16, 1, 2, 2, false, 2)
+SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 2, 2, false, 2)
+SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 1, 2, false, 2)
+SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 1, 2, false, 2)
+SEQ_INST(hat_attnseq_bf16_d1_gen, bf16, 1, 2, 2, true, 2)
+SEQ_INST(hat_attnseq_bf16_d2_gen, bf16, 2, 2, 2, true, 2)
+SEQ_INST(hat_attnseq_bf16_d3_gen, bf16, 3, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_bf16_d4_gen, bf16, 4, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_f32_d1, float, 1, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_f32_d2, float, 2, 1, 2, true, 2)
+SEQ_INST(hat_attnseq_f32_d3, float, 3, 1, 1, true, 2)
+SEQ_INST(hat_attnseq_f32_d4, float, 4, 1, 1, true, 2)
+
+#define SPLIT_INST(NAME, T, DT, W)                                                                           \
+    extern "C" __global__ __launch_bounds__(64 * W, 1) void NAME(SeqAttnArgs p)                              \
+    {                                                                                                        \
+        constexpr int B = SplitShape<T, DT, W>::BYTES;                                                       \
+        __shared__ __attribute__((aligned(16))) unsigned char B0[B], B1[B], B2[B], B3[B];                    \
+        __shared__ __attribute__((aligned(16))) unsigned P0[W * 128], P1[W * 128];                           \
+        __shared__ float ml[W * 64];                                                                         \
+        __shared__ unsigned flags;                                                                           \
+        seq_split_body<T, DT, W>(p, B0, B1, B2, B3, P0, P1, ml, &flags);                                     \
+    }
+
+SPLIT_INST(hat_attnseq_f16_d1_split, f16, 1, 4)
+SPLIT_INST(hat_attnseq_f16_d2_split, f16, 2, 4)
+SPLIT_INST(hat_attnseq_f16_d3_split, f16, 3, 4)
+SPLIT_INST(hat_attnseq_f16_d4_split, f16, 4, 4)
+SPLIT_INST(hat_attnseq_bf16_d1_split, bf16, 1, 4)
+SPLIT_INST(hat_attnseq_bf16_d2_split, bf16, 2, 4)
+SPLIT_INST(hat_attnseq_bf16_d3_split, bf16, 3, 4)
+SPLIT_INST(hat_attnseq_bf16_d4_split, bf16, 4, 4)
+SPLIT_INST(hat_attnseq_f32_d1_split, float, 1, 4)
+SPLIT_INST(hat_attnseq_f32_d2_split, float, 2, 4)
+SPLIT_INST(hat_attnseq_f32_d3_split, float, 3, 2)
+SPLIT_INST(hat_attnseq_f32_d4_split, float, 4, 2)
+
+#define JOIN_INST(NAME, T) \
+    extern "C" __global__ __launch_bounds__(256) void NAME(SeqAttnArgs p) { seq_join_body<T>(p); }
+
+JOIN_INST(hat_attnseq_join_f32, float)
+JOIN_INST(hat_attnseq_join_f16, f16)
+JOIN_INST(hat_attnseq_join_bf16, bf16)

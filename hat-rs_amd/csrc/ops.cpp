@@ -210,6 +210,7 @@ void check_attention(const hat_attention* a)
                     std::to_string(a->kv_heads) + " key heads");
     check_range(op, "q_tokens", a->q_tokens, 0, (1ll << 31) - 1024);
     check_range(op, "k_tokens", a->k_tokens, 0, (1ll << 31) - 1024);
+    check_range(op, "q_tokens times heads", a->q_tokens * (a->q_heads / a->kv_heads), 0, (1ll << 31) - 1024);
     if (!std::isfinite(a->scale)) throw Error("attention: scale must be finite");
     if (!(a->cap >= 0.0f) || !std::isfinite(a->cap)) throw Error("attention: cap must be 0 or positive");
     if ((a->cu_q && a->q_lens) || (a->cu_k && a->k_lens))
@@ -224,10 +225,54 @@ void check_attention(const hat_attention* a)
 
 }  // namespace
 
+namespace {
+
+// How a call runs, from its sizes alone.
+struct AttnPlan {
+    bool split;       // keys in chunks over blocks and waves
+    int tiles;        // of rows: a sequence's (batch) or all sequences' slots (packed)
+    int chunk, slots; // split: keys a chunk; a sequence's chunks (batch) or all slots (packed)
+    long long blocks, join_rows;  // join_rows > 0: partial results and their join
+    size_t workspace;
+};
+
+int dim_tiles(const hat_attention* a) { return (a->head_dim + 31) / 32; }
+
+AttnPlan attn_plan(const hat_attention* a)
+{
+    AttnPlan p{};
+    const int group = a->q_heads / a->kv_heads;
+    const long long rows = a->q_tokens * group;
+    p.split = !a->cu_q && rows <= 64;
+    if (p.split) {
+        p.tiles = (int)((rows + 31) / 32);
+        // Enough chunks that every CU has two blocks, of 256 keys at least.
+        const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
+        const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
+        p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / 512 + 127) / 128 * 128));
+        const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
+        const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
+        p.slots = (int)(a->cu_k ? slots : std::max<long long>(n, 1));
+        p.blocks = slots * a->kv_heads * p.tiles;
+        if (n > 1) {
+            p.join_rows = rows * a->kv_heads * a->n_seq;
+            p.workspace = (size_t)(slots * a->kv_heads * rows) * (a->head_dim + 2) * sizeof(float);
+        }
+    } else {
+        const int per = dim_tiles(a) <= 2 && a->dtype != HAT_F32 ? 256 : 128;  // rows a block (SEQ_INST)
+        const long long tiles = a->cu_q ? rows / per + a->n_seq : (rows + per - 1) / per;
+        p.blocks = tiles * a->kv_heads * (a->cu_q ? 1 : a->n_seq);
+        p.tiles = (int)tiles;
+    }
+    return p;
+}
+
+}  // namespace
+
 size_t op_attention_workspace(const hat_attention* a)
 {
     check_attention(a);
-    return 0;
+    return a->n_seq == 0 || a->q_tokens == 0 ? 0 : attn_plan(a).workspace;
 }
 
 void op_attention(const hat_attention* a, void* stream)
@@ -250,6 +295,12 @@ void op_attention(const hat_attention* a, void* stream)
     for (const void* i : {(const void*)a->cu_q, (const void*)a->cu_k, (const void*)a->q_lens, (const void*)a->k_lens,
                           (const void*)a->prefix, (const void*)a->slopes})
         if (i) check_pointer(op, "an int32 or fp32 argument", i, 4);
+    const AttnPlan plan = attn_plan(a);
+    if (plan.workspace) {
+        if (!a->workspace || a->workspace_bytes < plan.workspace)
+            throw Error("attention: a workspace of " + std::to_string(plan.workspace) + " bytes is needed");
+        if ((uintptr_t)a->workspace % 16) throw Error("attention: the workspace is not aligned to 16 bytes");
+    }
     SeqAttnArgs p{};
     p.q = a->q.data, p.k = a->k.data, p.v = a->v.data, p.o = a->out.data;
     p.qb = a->q.batch_stride, p.qt = a->q.token_stride, p.qh = a->q.head_stride;
@@ -267,12 +318,35 @@ void op_attention(const hat_attention* a, void* stream)
     p.dim = a->head_dim;
     p.q_tokens = (int)a->q_tokens, p.k_tokens = (int)a->k_tokens;
     p.causal = a->causal != 0;
+    // Rows in 16-byte chunks: aligned, a head of whole chunks, and a stage of 64 rows
+    // within a buffer descriptor's 31 bits.
+    const int size = (int)element(a->dtype);
+    const long long far = (1ll << 24) / size;
+    p.wide = a->head_dim * size % 16 == 0 && aligned(a->q, a->dtype, 16) && aligned(a->k, a->dtype, 16) &&
+             aligned(a->v, a->dtype, 16) && a->k.token_stride < far && a->v.token_stride < far;
+    p.wide_out = a->head_dim % 4 == 0 && aligned(a->out, a->dtype, 4 * size);
     p.scale = a->scale;
     p.cap = a->cap, p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
+    // positive (the sign goes into q), so that the largest score is the largest product
+    const double c = std::max(std::fabs((double)a->scale), 1e-37) * LOG2E;
+    p.c1 = (float)(a->cap > 0.0f ? 2.0 * c / a->cap : c);
+    p.tiles = plan.tiles, p.chunk = plan.chunk, p.slots = plan.slots;
+    if (plan.join_rows) {
+        p.part = (float*)a->workspace;
+        p.part_ml = p.part + plan.workspace / sizeof(float) / (a->head_dim + 2) * a->head_dim;
+    }
     const DeviceScope scope;
     hipStream_t s = check_stream(op, stream);
-    const long long rows = a->q_tokens * a->q_heads * (a->cu_q ? 1 : a->n_seq);
-    launch(s, (std::string("hat_attnseq_rows_") + type_name(a->dtype)).c_str(), grid_of(op, (rows + 3) / 4), 1, 1, 256, p);
+    const std::string type = type_name(a->dtype);
+    std::string name = "hat_attnseq_" + type + "_d" + std::to_string(dim_tiles(a));
+    if (plan.split)
+        name += "_split";
+    else if (a->dtype != HAT_F32 && (a->cap > 0.0f || a->slopes))
+        name += "_gen";
+    const int threads = plan.split && a->dtype == HAT_F32 && dim_tiles(a) > 2 ? 128 : 256;
+    launch(s, name.c_str(), grid_of(op, plan.blocks), 1, 1, threads, p);
+    if (plan.join_rows)
+        launch(s, ("hat_attnseq_join_" + type).c_str(), grid_of(op, (plan.join_rows + 3) / 4), 1, 1, 256, p);
 }
 
 // ---------------------------------------------------------------------------
