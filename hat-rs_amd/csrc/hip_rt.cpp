@@ -38,20 +38,26 @@ const std::vector<std::string>& required_kernels()
         "hat_rotary_f32_v4", "hat_rotary_f32_v2", "hat_rotary_f32_v1", "hat_rotary_f16_v8", "hat_rotary_f16_v4",
         "hat_rotary_f16_v1", "hat_rotary_bf16_v8", "hat_rotary_bf16_v4", "hat_rotary_bf16_v1",
         "hat_attnseq_f16_d1", "hat_attnseq_f16_d2", "hat_attnseq_f16_d3", "hat_attnseq_f16_d4",
-        "hat_attnseq_f16_d1_gen", "hat_attnseq_f16_d2_gen", "hat_attnseq_f16_d3_gen", "hat_attnseq_f16_d4_gen",
+        "hat_attnseq_f16_d1_bias", "hat_attnseq_f16_d2_bias", "hat_attnseq_f16_d3_bias", "hat_attnseq_f16_d4_bias",
+        "hat_attnseq_f16_d1_cap", "hat_attnseq_f16_d2_cap", "hat_attnseq_f16_d3_cap", "hat_attnseq_f16_d4_cap",
+        "hat_attnseq_f16_d1_both", "hat_attnseq_f16_d2_both", "hat_attnseq_f16_d3_both", "hat_attnseq_f16_d4_both",
         "hat_attnseq_f16_d1_split", "hat_attnseq_f16_d2_split", "hat_attnseq_f16_d3_split", "hat_attnseq_f16_d4_split",
         "hat_attnseq_bf16_d1", "hat_attnseq_bf16_d2", "hat_attnseq_bf16_d3", "hat_attnseq_bf16_d4",
-        "hat_attnseq_bf16_d1_gen", "hat_attnseq_bf16_d2_gen", "hat_attnseq_bf16_d3_gen", "hat_attnseq_bf16_d4_gen",
+        "hat_attnseq_bf16_d1_bias", "hat_attnseq_bf16_d2_bias", "hat_attnseq_bf16_d3_bias", "hat_attnseq_bf16_d4_bias",
+        "hat_attnseq_bf16_d1_cap", "hat_attnseq_bf16_d2_cap", "hat_attnseq_bf16_d3_cap", "hat_attnseq_bf16_d4_cap",
+        "hat_attnseq_bf16_d1_both", "hat_attnseq_bf16_d2_both", "hat_attnseq_bf16_d3_both", "hat_attnseq_bf16_d4_both",
         "hat_attnseq_bf16_d1_split", "hat_attnseq_bf16_d2_split", "hat_attnseq_bf16_d3_split", "hat_attnseq_bf16_d4_split",
         "hat_attnseq_f32_d1", "hat_attnseq_f32_d2", "hat_attnseq_f32_d3", "hat_attnseq_f32_d4",
+        "hat_attnseq_f32_d1_bias", "hat_attnseq_f32_d2_bias", "hat_attnseq_f32_d3_bias", "hat_attnseq_f32_d4_bias",
+        "hat_attnseq_f32_d1_both", "hat_attnseq_f32_d2_both", "hat_attnseq_f32_d3_both", "hat_attnseq_f32_d4_both",
         "hat_attnseq_f32_d1_split", "hat_attnseq_f32_d2_split", "hat_attnseq_f32_d3_split", "hat_attnseq_f32_d4_split",
         "hat_attnseq_join_f32", "hat_attnseq_join_f16", "hat_attnseq_join_bf16",
         "hat_resnorm_f32_16", "hat_resnorm_f32_64", "hat_resnorm_f32_256", "hat_resnorm_f32_1024",
         "hat_resnorm_f32_64e", "hat_resnorm_f32_1024e",
         "hat_resnorm_f16_16", "hat_resnorm_f16_64", "hat_resnorm_f16_256", "hat_resnorm_f16_1024",
-        "hat_resnorm_f16_64e", "hat_resnorm_f16_1024e",
+        "hat_resnorm_f16_64h", "hat_resnorm_f16_1024h", "hat_resnorm_f16_64e", "hat_resnorm_f16_1024e",
         "hat_resnorm_bf16_16", "hat_resnorm_bf16_64", "hat_resnorm_bf16_256", "hat_resnorm_bf16_1024",
-        "hat_resnorm_bf16_64e", "hat_resnorm_bf16_1024e",
+        "hat_resnorm_bf16_64h", "hat_resnorm_bf16_1024h", "hat_resnorm_bf16_64e", "hat_resnorm_bf16_1024e",
     };
     return k;
 }

@@ -400,7 +400,7 @@ struct SeqAttnArgs {
     long long pqb, pqt, pqa, pkb, pkt, pka;
     int n_seq, q_heads, kv_heads, group, dim, axes;
     int q_tokens, k_tokens;  // of a batch entry, or of the packed tensor
-    int causal;
+    int causal, fold;
     int wide;                // q, k, v rows: 16-byte chunks (else element by element)
     int wide_out;            // out rows: four elements at a time
     float scale;             // scores = scale * q . k

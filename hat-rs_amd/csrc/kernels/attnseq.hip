@@ -171,6 +171,17 @@ __device__ __forceinline__ unsigned pack16(float a, float b, f16)
 }
 __device__ __forceinline__ unsigned pack16(float a, float b, bf16) { return pk_bf16(a, b); }
 
+// s plus both values of a packed pair: the sum is over the probabilities that the
+// product with v sees.
+__device__ __forceinline__ float add_pair(unsigned w, float s, f16)
+{
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), (f16x2){(_Float16)1.0f, (_Float16)1.0f}, s, false);
+}
+__device__ __forceinline__ float add_pair(unsigned w, float s, bf16)
+{
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, s, false);
+}
+
 // The rows of K or V of one stage into LDS, by THREADS threads (a block, or one wave on
 // its own): R rows from row `first` of n, zeros past the last and past the head's dims.
 // Chunks go straight to LDS through a buffer descriptor that ends with the last row,
@@ -278,18 +289,27 @@ struct SeqAcc {
     }
 };
 
+// What stands between q . k and the softmax, compiled apart: every instruction a score
+// costs counts, as the vector and the matrix unit take turns.
+enum SeqMode {
+    SEQ_PLAIN,  // nothing
+    SEQ_BIAS,   // the bias, which MFMA's accumulator starts from (in units of q . k)
+    SEQ_CAP,    // the cap: scores held as r = 1 / (e^2x + 1), tanh x = 1 - 2 r
+    SEQ_BOTH,   // whatever the arguments say, in log2 units
+};
+
 // The bias of a lane's row.
 struct SeqBias {
-    float slope;      // log2 units
+    float slope;      // SEQ_BIAS: in units of q . k; SEQ_BOTH: in log2 units
     int at;           // i + Lk - Lq
     unsigned pos[4];  // positions, offset to order as unsigned
 };
 
-template <class T>
-__device__ __forceinline__ SeqBias seq_bias(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r)
+__device__ __forceinline__ SeqBias seq_bias(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r, bool raw)
 {
     SeqBias b;
     b.slope = p.slopes && r.live ? p.slopes[r.head] * HAT_LOG2E : 0.0f;
+    if (raw) b.slope /= p.c1;
     b.at = r.i + v.lk - v.lq;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -300,14 +320,74 @@ __device__ __forceinline__ SeqBias seq_bias(const SeqAttnArgs& p, const SeqView&
     return b;
 }
 
-// The scores of 32 keys from k0 in log2 units: the cap and the bias on q . k. pk: the
-// keys' positions in LDS, one row of `pstride` an axis. Register r is key
-// 8 (r / 4) + 4 h + r % 4.
+// c + |a - b|: one instruction, which the compiler does not form by itself.
+__device__ __forceinline__ unsigned sad(unsigned a, unsigned b, unsigned c)
+{
+    unsigned d;
+    asm("v_sad_u32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+// s[r] -= slope * distance for 32 keys by their positions in LDS (pk, one row of `pstride`
+// an axis). Register r is key 8 (r / 4) + 4 h + r % 4.
+__device__ __forceinline__ void pos_bias(const SeqAttnArgs& p, const SeqBias& b, f32x16& s, const unsigned* pk, int pstride)
+{
+    const unsigned* k = pk + 4 * ((threadIdx.x >> 5) & 1);
+    unsigned far[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) far[r] = 0;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        if (a < p.axes) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const u32x4 x = *(const u32x4*)(k + a * pstride + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) far[4 * g + e] = sad(b.pos[a], x[e], far[4 * g + e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-b.slope, (float)far[r], s[r]);
+}
+
+__device__ __forceinline__ void index_bias(const SeqBias& b, f32x16& s, int k0)
+{
+    const float at = (float)(b.at - k0 - 4 * (int)((threadIdx.x >> 5) & 1));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-b.slope, fabsf(at - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+}
+
+// Where MFMA starts from for 32 keys from k0: s, and a row's constant beside it. By index,
+// keys that lie on one side of all the wave's rows (at0 .. at1) have a bias that is linear
+// in the key: a product with the key's place in the tile, the rest a constant of the row.
+template <int MODE>
+__device__ __forceinline__ float seq_start(const SeqAttnArgs& p, const SeqBias& b, f32x16& s, int k0, const unsigned* pk,
+                                           int pstride, int at0, int at1)
+{
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    if constexpr (MODE != SEQ_BIAS) return 0.0f;
+    if (p.pos_q) {
+        pos_bias(p, b, s, pk, pstride);
+        return 0.0f;
+    }
+    if (k0 + 31 <= at0 || k0 >= at1) {
+        const float sl = k0 >= at1 ? -b.slope : b.slope;
+        const float base = (float)(4 * (int)((threadIdx.x >> 5) & 1));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = sl * (float)(8 * (r >> 2) + (r & 3));
+        return sl * ((float)(k0 - b.at) + base);
+    }
+    index_bias(b, s, k0);
+    return 0.0f;
+}
+
+// SEQ_BOTH: the scores of 32 keys from k0 in log2 units.
 template <class T>
 __device__ __forceinline__ void seq_scores(const SeqAttnArgs& p, const SeqBias& b, f32x16& s, int k0, const unsigned* pk,
                                            int pstride)
 {
-    const int h = (threadIdx.x >> 5) & 1;
     if (p.cap > 0.0f) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -325,49 +405,21 @@ __device__ __forceinline__ void seq_scores(const SeqAttnArgs& p, const SeqBias& 
         for (int r = 0; r < 16; ++r) s[r] *= p.c1;
     }
     if (!p.slopes) return;
-    if (!p.pos_q) {
-        const float at = (float)(b.at - k0 - 4 * h);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-b.slope, fabsf(at - (float)(8 * (r >> 2) + (r & 3))), s[r]);
-    } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            unsigned far[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                if (a < p.axes) {
-                    const u32x4 k = *(const u32x4*)(pk + a * pstride + 8 * g + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) far[e] += max(b.pos[a], k[e]) - min(b.pos[a], k[e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_fmaf(-b.slope, (float)far[e], s[4 * g + e]);
-        }
-    }
+    if (p.pos_q)
+        pos_bias(p, b, s, pk, pstride);
+    else
+        index_bias(b, s, k0);
 }
 
-// One stage of KT x 32 keys for QT x 32 rows of a wave: S^T = K Q^T (A = 32 keys, B =
-// the wave's q), so that a lane holds 16 scores of one row and, as probabilities, the B
-// operand of O^T += V^T P^T without a move. With MFMA's key order within 16 (lane half h,
-// slot j: keys 4 h + j, then 8 + 4 h + j - 4) V's operand is two transposed reads of
-// four keys each. The running maximum moves only when a score passes it by 2^8, so the
-// sums are seldom rescaled; P stays below 2^8.
-template <class T, int DT, int QT, int KT, bool GEN>
-__device__ __forceinline__ void seq_stage(const SeqAttnArgs& p, const unsigned char* K, const unsigned char* V,
-                                          const unsigned* pk, int pstride, const u32x4 (&q)[QT][SeqShape<T, DT>::KS],
-                                          SeqAcc<T, DT> (&acc)[QT], const SeqBias (&bias)[QT], const int (&limit)[QT],
-                                          int k0, bool masked)
+// S^T = K Q^T of KT x 32 keys and QT x 32 rows (A = 32 keys, B = the wave's q), so that
+// a lane holds 16 scores of one row and, as probabilities, the B operand of O^T += V^T P^T
+// without a move. s: where it starts from.
+template <class T, int DT, int QT, int KT>
+__device__ __forceinline__ void seq_qk(const unsigned char* K, const u32x4 (&q)[QT][SeqShape<T, DT>::KS],
+                                       f32x16 (&s)[QT][KT])
 {
     using S = SeqShape<T, DT>;
     const int lane = threadIdx.x & 63, ql = lane & 31, h = lane >> 5;
-    f32x16 s[QT][KT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][kt][r] = 0.0f;
     const int krow = ql * S::ROW, ksw = S::kswz(ql);
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
@@ -387,24 +439,44 @@ __device__ __forceinline__ void seq_stage(const SeqAttnArgs& p, const unsigned c
             }
         }
     }
-    u32x4 pb[QT][KT][2];  // 16-bit types: P packed, 16 keys each
+}
+
+// The mask and the running maximum: it moves only when a score passes it by 2^8, so the
+// sums are seldom rescaled; P stays below 2^8. rc: the rows' constants (seq_start).
+template <class T, int DT, int QT, int KT, int MODE>
+__device__ __forceinline__ void seq_max(const SeqAttnArgs& p, const unsigned* pk, int pstride, f32x16 (&s)[QT][KT],
+                                        const float (&rc)[QT][KT], SeqAcc<T, DT> (&acc)[QT], const SeqBias (&bias)[QT],
+                                        const int (&limit)[QT], int k0, bool masked)
+{
+    const int h = (threadIdx.x >> 5) & 1;
+    const float a = p.cap * HAT_LOG2E;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         SeqAcc<T, DT>& c = acc[t];
         float mx = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            if constexpr (GEN) seq_scores<T>(p, bias[t], s[t][kt], k0 + 32 * kt, pk + 32 * kt, pstride);
+            f32x16& x = s[t][kt];
+            if constexpr (MODE == SEQ_BOTH) seq_scores<T>(p, bias[t], x, k0 + 32 * kt, pk + 32 * kt, pstride);
+            if constexpr (MODE == SEQ_CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_rcpf(fast_exp2(x[r] * p.c1) + 1.0f);
+            }
             if (masked) {
+                const float out = MODE == SEQ_CAP ? INFINITY : -INFINITY;
                 const int left = limit[t] - k0 - 32 * kt - 4 * h;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[t][kt][r] = 8 * (r >> 2) + (r & 3) < left ? s[t][kt][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + (r & 3) < left ? x[r] : out;
             }
+            float m = x[0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][kt][r]);
+            for (int r = 1; r < 16; ++r) m = MODE == SEQ_CAP ? fminf(m, x[r]) : fmaxf(m, x[r]);
+            if constexpr (MODE == SEQ_CAP) m = __builtin_fmaf(-2.0f * a, m, a);
+            if constexpr (MODE == SEQ_BIAS) m += rc[t][kt];
+            mx = fmaxf(mx, m);
         }
         mx = swap_max(mx);
-        if constexpr (!GEN) mx *= p.c1;
+        if constexpr (MODE == SEQ_PLAIN || MODE == SEQ_BIAS) mx *= p.c1;
         if (__any(mx > c.m + 8.0f)) {
             const float mn = fmaxf(c.m, mx), corr = fast_exp2(c.m - mn);
             c.m = mn;
@@ -414,20 +486,47 @@ __device__ __forceinline__ void seq_stage(const SeqAttnArgs& p, const unsigned c
 #pragma unroll
                 for (int r = 0; r < 16; ++r) c.o[d][r] *= corr;
         }
+    }
+}
+
+// The probabilities 2^(s - m), in place (fp32) or packed for the product (16-bit types).
+template <class T, int DT, int QT, int KT, int MODE>
+__device__ __forceinline__ void seq_exp(const SeqAttnArgs& p, f32x16 (&s)[QT][KT], const float (&rc)[QT][KT],
+                                        SeqAcc<T, DT> (&acc)[QT], u32x4 (&pb)[QT][KT][2])
+{
+    const float a = p.cap * HAT_LOG2E;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        SeqAcc<T, DT>& c = acc[t];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
+            const float f = MODE == SEQ_CAP ? -2.0f * a : p.c1;
+            const float m = MODE == SEQ_CAP ? a - c.m : MODE == SEQ_BIAS ? __builtin_fmaf(rc[t][kt], p.c1, -c.m) : -c.m;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = fast_exp2(GEN ? s[t][kt][r] - c.m : __builtin_fmaf(s[t][kt][r], p.c1, -c.m));
-                s[t][kt][r] = e;
-                c.l += e;
+                s[t][kt][r] = fast_exp2(MODE == SEQ_BOTH ? s[t][kt][r] + m : __builtin_fmaf(s[t][kt][r], f, m));
+                if constexpr (sizeof(T) == 4) c.l += s[t][kt][r];
             }
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int r = 0; r < 16; r += 2) pb[t][kt][r >> 3][(r & 7) >> 1] = pack16(s[t][kt][r], s[t][kt][r + 1], T());
+                for (int r = 0; r < 16; r += 2) {
+                    const unsigned w = pack16(s[t][kt][r], s[t][kt][r + 1], T());
+                    pb[t][kt][r >> 3][(r & 7) >> 1] = w;
+                    c.l = add_pair(w, c.l, T());
+                }
             }
         }
     }
+}
+
+// O^T += V^T P^T. With MFMA's key order within 16 (lane half h, slot j: keys 4 h + j,
+// then 8 + 4 h + j - 4) V's 16-bit operand is two transposed reads of four keys each.
+template <class T, int DT, int QT, int KT>
+__device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)[QT][KT], const u32x4 (&pb)[QT][KT][2],
+                                       SeqAcc<T, DT> (&acc)[QT])
+{
+    using S = SeqShape<T, DT>;
+    const int lane = threadIdx.x & 63, ql = lane & 31, h = lane >> 5;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -513,7 +612,7 @@ __device__ __forceinline__ SeqView uniform(const SeqView& v)
 
 // ---- many rows: a block of four waves, QT x 32 rows each, walks the keys in stages of
 // KT x 32, two in LDS: the next one's copy runs under the present one's products.
-template <class T, int DT, int QT, int KT, bool GEN>
+template <class T, int DT, int QT, int KT, int MODE>
 __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0, unsigned char* K1, unsigned char* V0,
                                          unsigned char* V1, unsigned* P0, unsigned* P1)
 {
@@ -536,7 +635,13 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
     const int rows = v.lq * p.group;
     const int tiles = (rows + BQ - 1) / BQ;
     if (tile >= tiles) return;
-    if (p.causal) tile = tiles - 1 - tile;  // the longest first
+    // Under the causal mask a tile's work grows with its number: the longest first, and
+    // where all blocks run at once (p.fold) the second half from the shortest on, so that
+    // the CUs, which take blocks in turn, get a long and a short one each.
+    if (p.causal) {
+        const int half = (tiles + 1) / 2;
+        tile = p.fold && tile >= half ? tile - half : tiles - 1 - tile;
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
     const int row0 = tile * BQ + wave * 32 * QT;
@@ -553,7 +658,7 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
         row[t] = seq_row(p, row0 + 32 * t + (lane & 31), rows, kvh);
         load_q<T, DT>(p, v, row[t], q[t]);
         limit[t] = row[t].live ? row_limit(p, v, row[t].i, prefix) : 0x7fffffff;
-        if constexpr (GEN) bias[t] = seq_bias<T>(p, v, row[t]);
+        if constexpr (MODE == SEQ_BIAS || MODE == SEQ_BOTH) bias[t] = seq_bias(p, v, row[t], MODE == SEQ_BIAS);
         acc[t].init();
     }
     // limits rise with the row: the wave's least and largest
@@ -569,30 +674,48 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
     sk.init((const T*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + kvh * p.kh, p.kt, v.lk, p.dim, tid);
     sv.init((const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + kvh * p.vh, p.vt, v.lk, p.dim, tid);
     const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
-    const auto issue = [&](unsigned char* K, unsigned char* V, unsigned* P, int k0) {
+    const int at0 = row0 / p.group + v.lk - v.lq, at1 = (row0 + 32 * QT - 1) / p.group + v.lk - v.lq;
+    const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
+        if (k0 >= most) return;
+        f32x16 s[QT][KT];
+        float rc[QT][KT];
+        u32x4 pb[QT][KT][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+                rc[t][kt] = seq_start<MODE>(p, bias[t], s[t][kt], k0 + 32 * kt, P + 32 * kt, BK, at0, at1);
+        seq_qk<T, DT, QT, KT>(K, q, s);
+        seq_max<T, DT, QT, KT, MODE>(p, P, BK, s, rc, acc, bias, limit, k0, k0 + BK > least);
+        seq_exp<T, DT, QT, KT, MODE>(p, s, rc, acc, pb);
+        seq_pv<T, DT, QT, KT>(V, s, pb, acc);
+    };
+    // The positions of a stage's keys, one a thread: read with the stage's copies, put into
+    // LDS behind the present stage's products.
+    const bool has_pos = (MODE == SEQ_BIAS || MODE == SEQ_BOTH) && p.pos_q && tid < p.axes * BK;
+    unsigned pos = 0;
+    const auto issue = [&](unsigned char* K, unsigned char* V, int k0) {
+        if (has_pos && k0 + tid % BK < v.lk)
+            pos = (unsigned)pos_k[(long long)(k0 + tid % BK) * p.pkt + tid / BK * p.pka] ^ 0x80000000u;
         sk.issue(K, k0, tid, p.wide);
         sv.issue(V, k0, tid, p.wide);
-        if constexpr (GEN) {
-            if (p.pos_q)
-                for (int e = tid; e < p.axes * BK; e += 256) {
-                    const int a = e / BK, j = k0 + e % BK;
-                    P[e] = j < v.lk ? (unsigned)pos_k[(long long)j * p.pkt + a * p.pka] ^ 0x80000000u : 0u;
-                }
-        }
     };
-    const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
-        if (k0 < most) seq_stage<T, DT, QT, KT, GEN>(p, K, V, P, BK, q, acc, bias, limit, k0, k0 + BK > least);
+    const auto put_pos = [&](unsigned* P) {
+        if (has_pos) P[tid] = pos;
     };
     if (end > 0) {
-        issue(K0, V0, P0, 0);
+        issue(K0, V0, 0);
+        put_pos(P0);
         __syncthreads();
         for (int k0 = 0; k0 < end; k0 += 2 * BK) {
-            issue(K1, V1, P1, k0 + BK);  // past the last key: zeros
+            issue(K1, V1, k0 + BK);  // past the last key: zeros
             stage(K0, V0, P0, k0);
+            put_pos(P1);
             __syncthreads();
             if (k0 + BK >= end) break;
-            issue(K0, V0, P0, k0 + 2 * BK);
+            issue(K0, V0, k0 + 2 * BK);
             stage(K1, V1, P1, k0 + BK);
+            put_pos(P0);
             __syncthreads();
         }
     }
@@ -663,19 +786,25 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
 {
     using X = SplitShape<T, DT, W>;
     constexpr int DP = 32 * DT;
-    // b = (slot * kv_heads + kvh) * tiles + tile
-    const int tile = blockIdx.x % p.tiles;
-    const int kvh = blockIdx.x / p.tiles % p.kv_heads;
-    const int slot = blockIdx.x / p.tiles / p.kv_heads;
-    int sq, chunk;
-    if (p.cu_k) {
-        int first = 0;
-        sq = find_sequence(p.cu_k, p.n_seq, p.k_tokens, 1, p.chunk, slot, first);
+    int tile, kvh, slot = 0, sq, chunk = 0, first = 0;
+    if (p.cu_q) {  // b = tile slot * kv_heads + kvh, all keys in one chunk
+        kvh = blockIdx.x % p.kv_heads;
+        tile = blockIdx.x / p.kv_heads;
+        sq = find_sequence(p.cu_q, p.n_seq, p.q_tokens, p.group, 32, tile, first);
         if (sq < 0) return;
-        chunk = slot - first;
-    } else {
-        sq = slot / p.slots;
-        chunk = slot - sq * p.slots;
+        tile = __builtin_amdgcn_readfirstlane(tile - first);
+    } else {  // b = (chunk slot * kv_heads + kvh) * tiles + tile
+        tile = blockIdx.x % p.tiles;
+        kvh = blockIdx.x / p.tiles % p.kv_heads;
+        slot = blockIdx.x / p.tiles / p.kv_heads;
+        if (p.cu_k) {
+            sq = find_sequence(p.cu_k, p.n_seq, p.k_tokens, 1, p.chunk, slot, first);
+            if (sq < 0) return;
+            chunk = slot - first;
+        } else {
+            sq = slot / p.slots;
+            chunk = slot - sq * p.slots;
+        }
     }
     const SeqView v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
     chunk = __builtin_amdgcn_readfirstlane(chunk);
@@ -697,7 +826,7 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     const SeqRow row = seq_row(p, row0 + (lane & 31), rows, kvh);
     load_q<T, DT>(p, v, row, q[0]);
     limit[0] = row.live ? row_limit(p, v, row.i, prefix) : 0x7fffffff;
-    bias[0] = seq_bias<T>(p, v, row);
+    bias[0] = seq_bias(p, v, row, false);
     acc[0].init();
 
     Stage<T, DT, 32, 64, false> sk;
@@ -707,32 +836,55 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
     const int lds = wave * X::TILE;
     constexpr int MOVES = 2 * Stage<T, DT, 32, 64, false>::N;
-    const auto issue = [&](unsigned char* K, unsigned char* V, unsigned* P, int k0) {
+    const auto issue = [&](unsigned char* K, unsigned char* V, int k0) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer's reads are done
         sk.issue(K + lds, k0, lane, p.wide);
         sv.issue(V + lds, k0, lane, p.wide);
-        if (p.pos_q)
-            for (int e = lane; e < p.axes * 32; e += 64) {
-                const int a = e >> 5, j = k0 + (e & 31);
-                P[wave * 128 + e] = j < c1 ? (unsigned)pos_k[(long long)j * p.pkt + a * p.pka] ^ 0x80000000u : 0u;
-            }
+    };
+    // The positions of a tile's keys, two axes a register: read with the tile's copies, put
+    // into LDS when the tile's turn comes.
+    unsigned pos[2] = {0, 0};
+    const auto read_pos = [&](int k0) {
+        const int j = k0 + (lane & 31);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int a = 2 * x + (lane >> 5);
+            if (p.pos_q && a < p.axes && j < c1) pos[x] = (unsigned)pos_k[(long long)j * p.pkt + a * p.pka] ^ 0x80000000u;
+        }
+    };
+    const auto put_pos = [&](unsigned* P) {
+        if (!p.pos_q) return;
+        P[wave * 128 + lane] = pos[0];
+        P[wave * 128 + 64 + lane] = pos[1];
     };
     const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
         // the other buffer's moves may still be under way
         if (p.wide) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOVES) : "memory");
         // limits end the chunk as well: keys behind it lie in another
-        seq_stage<T, DT, 1, 1, true>(p, K + lds, V + lds, P + wave * 128, 32, q, acc, bias, limit, k0,
-                                     k0 + 32 > least || k0 + 32 > c1);
+        f32x16 s[1][1];
+        const float rc[1][1] = {{0.0f}};
+        u32x4 pb[1][1][2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][0][r] = 0.0f;
+        seq_qk<T, DT, 1, 1>(K + lds, q, s);
+        seq_max<T, DT, 1, 1, SEQ_BOTH>(p, P + wave * 128, 32, s, rc, acc, bias, limit, k0, k0 + 32 > least || k0 + 32 > c1);
+        seq_exp<T, DT, 1, 1, SEQ_BOTH>(p, s, rc, acc, pb);
+        seq_pv<T, DT, 1, 1>(V + lds, s, pb, acc);
     };
     limit[0] = limit[0] < c1 ? limit[0] : c1;
     int k0 = c0 + 32 * wave;
-    issue(B0, B2, P0, k0);
+    read_pos(k0);
+    issue(B0, B2, k0);
     while (k0 < c1) {
-        issue(B1, B3, P1, k0 + 32 * W);
+        put_pos(P0);
+        read_pos(k0 + 32 * W);
+        issue(B1, B3, k0 + 32 * W);
         stage(B0, B2, P0, k0);
         k0 += 32 * W;
         if (k0 >= c1) break;
-        issue(B0, B2, P0, k0 + 32 * W);
+        put_pos(P1);
+        read_pos(k0 + 32 * W);
+        issue(B0, B2, k0 + 32 * W);
         stage(B1, B3, P1, k0);
         k0 += 32 * W;
     }
@@ -853,35 +1005,60 @@ __device__ __forceinline__ void seq_join_body(const SeqAttnArgs& p)
     if (lane + 64 < p.dim) o[lane + 64] = (T)(oc * join_scale(l));
 }
 
-#define SEQ_INST(NAME, T, DT, QT, KT, GEN, WPS)                                                              \
+#define SEQ_INST(NAME, T, DT, QT, KT, MODE, WPS)                                                             \
     extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
     {                                                                                                        \
         constexpr int B = 32 * KT * SeqShape<T, DT>::ROW;                                                    \
+        constexpr int PB = MODE == SEQ_BIAS || MODE == SEQ_BOTH ? 128 * KT : 4;                              \
         __shared__ __attribute__((aligned(16))) unsigned char K0[B], K1[B], V0[B], V1[B];                    \
-        __shared__ __attribute__((aligned(16))) unsigned P0[GEN ? 128 * KT : 4], P1[GEN ? 128 * KT : 4];     \
-        seq_body<T, DT, QT, KT, GEN>(p, K0, K1, V0, V1, P0, P1);                                             \
+        __shared__ __attribute__((aligned(16))) unsigned P0[PB], P1[PB];                                     \
+        seq_body<T, DT, QT, KT, MODE>(p, K0, K1, V0, V1, P0, P1);                                            \
     }
 
-SEQ_INST(hat_attnseq_f16_d1, f16, 1, 2, 2, false, 2)
-SEQ_INST(hat_attnseq_f16_d2, f16, 2, 2, 2, false, 2)
-SEQ_INST(hat_attnseq_f16_d3, f16, 3, 1, 2, false, 2)
-SEQ_INST(hat_attnseq_f16_d4, f16, 4, 1, 2, false, 2)
-SEQ_INST(hat_attnseq_f16_d1_gen, f16, 1, 2, 2, true, 2)
-SEQ_INST(hat_attnseq_f16_d2_gen, f16, 2, 2, 2, true, 2)
-SEQ_INST(hat_attnseq_f16_d3_gen, f16, 3, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_f16_d4_gen, f16, 4, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_bf16_d1, bf16, 1, 2, 2, false, 2)
-SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 2, 2, false, 2)
-SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 1, 2, false, 2)
-SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 1, 2, false, 2)
-SEQ_INST(hat_attnseq_bf16_d1_gen, bf16, 1, 2, 2, true, 2)
-SEQ_INST(hat_attnseq_bf16_d2_gen, bf16, 2, 2, 2, true, 2)
-SEQ_INST(hat_attnseq_bf16_d3_gen, bf16, 3, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_bf16_d4_gen, bf16, 4, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_f32_d1, float, 1, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_f32_d2, float, 2, 1, 2, true, 2)
-SEQ_INST(hat_attnseq_f32_d3, float, 3, 1, 1, true, 2)
-SEQ_INST(hat_attnseq_f32_d4, float, 4, 1, 1, true, 2)
+SEQ_INST(hat_attnseq_f16_d1, f16, 1, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_f16_d2, f16, 2, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_f16_d3, f16, 3, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f16_d4, f16, 4, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f16_d1_bias, f16, 1, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_f16_d2_bias, f16, 2, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_f16_d3_bias, f16, 3, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f16_d4_bias, f16, 4, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f16_d1_cap, f16, 1, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_f16_d2_cap, f16, 2, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_f16_d3_cap, f16, 3, 1, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_f16_d4_cap, f16, 4, 1, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_f16_d1_both, f16, 1, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d2_both, f16, 2, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d3_both, f16, 3, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d4_both, f16, 4, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d1, bf16, 1, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_bf16_d1_bias, bf16, 1, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_bf16_d2_bias, bf16, 2, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_bf16_d3_bias, bf16, 3, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_bf16_d4_bias, bf16, 4, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_bf16_d1_cap, bf16, 1, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_bf16_d2_cap, bf16, 2, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_bf16_d3_cap, bf16, 3, 1, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_bf16_d4_cap, bf16, 4, 1, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_bf16_d1_both, bf16, 1, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d2_both, bf16, 2, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d3_both, bf16, 3, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f32_d1, float, 1, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f32_d1_bias, float, 1, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f32_d1_both, float, 1, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f32_d2, float, 2, 1, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f32_d2_bias, float, 2, 1, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f32_d2_both, float, 2, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f32_d3, float, 3, 1, 1, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f32_d3_bias, float, 3, 1, 1, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f32_d3_both, float, 3, 1, 1, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f32_d4, float, 4, 1, 1, SEQ_PLAIN, 1)
+SEQ_INST(hat_attnseq_f32_d4_bias, float, 4, 1, 1, SEQ_BIAS, 1)
+SEQ_INST(hat_attnseq_f32_d4_both, float, 4, 1, 1, SEQ_BOTH, 1)
 
 #define SPLIT_INST(NAME, T, DT, W)                                                                           \
     extern "C" __global__ __launch_bounds__(64 * W, 1) void NAME(SeqAttnArgs p)                              \

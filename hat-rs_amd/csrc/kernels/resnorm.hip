@@ -28,44 +28,81 @@ __device__ __forceinline__ float row_sum(float v, float* lds)
     return v;
 }
 
-// v = N(v) over the row's p.width values.
+// A row of p.width elements: moves at the thread's vectors i * TPR + t. Rows that a whole
+// wave shares go through a buffer descriptor that ends with the row (zeros past it, no
+// branch); rows of 16 threads through pointers and a check a vector.
+template <class T, int TPR, int V>
+struct Row {
+    T* p;
+    __amdgpu_buffer_rsrc_t r;
+    int width, t;
+    __device__ __forceinline__ Row(const void* base, long long offset, int w, int thread) : width(w), t(thread)
+    {
+        p = (T*)base + offset;
+        if constexpr (TPR >= 64) r = buffer_of(p, w * (int)sizeof(T));
+    }
+    __device__ __forceinline__ void load(int i, float (&v)[V]) const
+    {
+        if constexpr (TPR >= 64) {
+            constexpr int part = sizeof(T) * V > 16 ? 16 / (int)sizeof(T) : V;
+#pragma unroll
+            for (int h = 0; h < V; h += part) {
+                float u[part];
+                buffer_load_vec<T, part>(r, t * V * (int)sizeof(T), (i * TPR * V + h) * (int)sizeof(T), u);
+#pragma unroll
+                for (int j = 0; j < part; ++j) v[h + j] = u[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = 0.0f;
+            if ((i * TPR + t) * V < width) load_vec<T, V>(p + (i * TPR + t) * V, v);
+        }
+    }
+    __device__ __forceinline__ void store(int i, const float (&v)[V]) const
+    {
+        if constexpr (TPR >= 64) {
+            buffer_store_vec<T, V>(r, t * V * (int)sizeof(T), i * TPR * V * (int)sizeof(T), v);
+        } else {
+            if ((i * TPR + t) * V < width) store_vec<T, V>(p + (i * TPR + t) * V, v);
+        }
+    }
+};
+
+// v = N(v) over the row's p.width values; zeros stay past the width.
 template <int TPR, int V, int NV>
 __device__ __forceinline__ void row_norm(float (&v)[NV][V], int kind, const float* w, const float* b, float eps,
                                          int width, int t, float* lds)
 {
-    float mean = 0.0f;
     if (kind == NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += v[i][j];  // zeros past the width
-        mean = row_sum<TPR>(s, lds) / (float)width;
+            for (int j = 0; j < V; ++j) s += v[i][j];
+        const float mean = row_sum<TPR>(s, lds) / (float)width;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float m = (i * TPR + t) * V < width ? mean : 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][j] -= m;
+        }
     }
     float q = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if ((i * TPR + t) * V < width) {
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[i][j] -= mean;
-                q = __builtin_fmaf(v[i][j], v[i][j], q);
-            }
-        }
-    }
+        for (int j = 0; j < V; ++j) q = __builtin_fmaf(v[i][j], v[i][j], q);
     const float r = 1.0f / sqrtf(row_sum<TPR>(q, lds) / (float)width + eps);
+    const Row<float, TPR, V> rw(w, 0, width, t), rb(b, 0, width, t);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * V;
-        if (c < width) {
-            float f[V], a[V];
+        float f[V], a[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) f[j] = 1.0f, a[j] = 0.0f;
-            if (w) load_vec<float, V>(w + c, f);
-            if (b) load_vec<float, V>(b + c, a);
+        for (int j = 0; j < V; ++j) f[j] = 1.0f, a[j] = 0.0f;
+        if (w) rw.load(i, f);
+        if (b) rb.load(i, a);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] = __builtin_fmaf(v[i][j] * r, f[j], a[j]);
-        }
+        for (int j = 0; j < V; ++j) v[i][j] = __builtin_fmaf(v[i][j] * r, f[j], a[j]);
     }
 }
 
@@ -75,54 +112,52 @@ __device__ __forceinline__ void resnorm_body(const ResNormArgs& p)
 {
     __shared__ float lds[THREADS / 64];
     const int t = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+    int in_block = threadIdx.x / TPR;
+    if constexpr (TPR >= 64) in_block = __builtin_amdgcn_readfirstlane(in_block);
+    const long long row = (long long)blockIdx.x * (THREADS / TPR) + in_block;
     if (row >= p.rows) return;  // whole rows leave; with more than a wave a row, whole blocks
     float v[NV][V];
     if (p.y) {
-        const T* y = (const T*)p.y + row * p.ys;
+        const Row<T, TPR, V> y(p.y, row * p.ys, p.width, t);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
-            if ((i * TPR + t) * V < p.width) load_vec<T, V>(y + (i * TPR + t) * V, v[i]);
-        }
+        for (int i = 0; i < NV; ++i) y.load(i, v[i]);
         if (p.post != NORM_NONE) row_norm<TPR, V, NV>(v, p.post, p.post_w, p.post_b, p.post_eps, p.width, t, lds);
+        if (p.gate) {
+            const Row<T, TPR, V> g(p.gate, (p.rows_per_gate == p.rows ? 0 : row / p.rows_per_gate) * p.gs, p.width, t);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float f[V];
+                g.load(i, f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] *= f[j];
+            }
+        }
     }
-    const T* x = (const T*)p.x + row * p.xs;
-    const T* g = p.gate ? (const T*)p.gate + row / p.rows_per_gate * p.gs : nullptr;
+    const Row<T, TPR, V> x(p.x, row * p.xs, p.width, t), xo(p.xo, row * p.xos, p.width, t);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * V;
         float u[V];
+        x.load(i, u);
+        if (p.y) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) u[j] = 0.0f;
-        if (c < p.width) {
-            load_vec<T, V>(x + c, u);
-            if (p.y) {
-                float f[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) f[j] = 1.0f;
-                if (g) load_vec<T, V>(g + c, f);
-#pragma unroll
-                for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(p.scale * f[j], v[i][j], u[j]);
-            }
-            if (p.xo) store_vec<T, V>((T*)p.xo + row * p.xos + c, u);
+            for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(p.scale, v[i][j], u[j]);
         }
+        if (p.xo) xo.store(i, u);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = u[j];
     }
     if (!p.h) return;
     if (p.pre != NORM_NONE) row_norm<TPR, V, NV>(v, p.pre, p.pre_w, p.pre_b, p.pre_eps, p.width, t, lds);
+    const Row<T, TPR, V> h(p.h, row * p.hs, p.width, t);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * V;
-        if (c < p.width) store_vec<T, V>((T*)p.h + row * p.hs + c, v[i]);
-    }
+    for (int i = 0; i < NV; ++i) h.store(i, v[i]);
 }
 
 #define RESNORM_INST(NAME, T, THREADS, TPR, V, NV) \
     extern "C" __global__ __launch_bounds__(THREADS) void NAME(ResNormArgs p) { resnorm_body<T, THREADS, TPR, V, NV>(p); }
 
+// by the bytes of a move (16; 4 or one element where the rows' alignment or width allow
+// no more) and the threads a row
 RESNORM_INST(hat_resnorm_f32_16, float, 256, 16, 4, 3)
 RESNORM_INST(hat_resnorm_f32_64, float, 256, 64, 4, 4)
 RESNORM_INST(hat_resnorm_f32_256, float, 256, 256, 4, 4)
@@ -133,11 +168,15 @@ RESNORM_INST(hat_resnorm_f16_16, f16, 256, 16, 8, 2)
 RESNORM_INST(hat_resnorm_f16_64, f16, 256, 64, 8, 4)
 RESNORM_INST(hat_resnorm_f16_256, f16, 256, 256, 8, 4)
 RESNORM_INST(hat_resnorm_f16_1024, f16, 1024, 1024, 8, 2)
+RESNORM_INST(hat_resnorm_f16_64h, f16, 256, 64, 2, 8)
+RESNORM_INST(hat_resnorm_f16_1024h, f16, 1024, 1024, 2, 8)
 RESNORM_INST(hat_resnorm_f16_64e, f16, 256, 64, 1, 16)
 RESNORM_INST(hat_resnorm_f16_1024e, f16, 1024, 1024, 1, 16)
 RESNORM_INST(hat_resnorm_bf16_16, bf16, 256, 16, 8, 2)
 RESNORM_INST(hat_resnorm_bf16_64, bf16, 256, 64, 8, 4)
 RESNORM_INST(hat_resnorm_bf16_256, bf16, 256, 256, 8, 4)
 RESNORM_INST(hat_resnorm_bf16_1024, bf16, 1024, 1024, 8, 2)
+RESNORM_INST(hat_resnorm_bf16_64h, bf16, 256, 64, 2, 8)
+RESNORM_INST(hat_resnorm_bf16_1024h, bf16, 1024, 1024, 2, 8)
 RESNORM_INST(hat_resnorm_bf16_64e, bf16, 256, 64, 1, 16)
 RESNORM_INST(hat_resnorm_bf16_1024e, bf16, 1024, 1024, 1, 16)

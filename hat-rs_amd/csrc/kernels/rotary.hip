@@ -16,6 +16,8 @@ using namespace hatk;
 
 #define ROT_THREADS 256
 #define ROT_ANGLES 4096  // cos and sin values a block keeps (32 KB)
+#define ROT_TOKENS 64    // tokens a block takes at most
+#define ROT_AHEAD 4
 
 // n / d for n < 2^20 by d's reciprocal: the error of (n + 1/2) / d is below 2^-2 / d.
 __device__ __forceinline__ int div_small(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
@@ -39,49 +41,81 @@ __device__ __forceinline__ void rotary_body(const RotaryArgs& p)
         cs[e] = c;
         sn[e] = s;
     }
+    // where the block's tokens lie in x and y
+    __shared__ long long at[4][ROT_TOKENS];
+    for (int t = threadIdx.x; t < n; t += ROT_THREADS) {
+        const long long b = (first + t) / p.tokens, tok = first + t - b * p.tokens;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            at[w][t] = b * p.xb[w] + tok * p.xt[w];
+            at[2 + w][t] = b * p.yb[w] + tok * p.yt[w];
+        }
+    }
     __syncthreads();
     const int turned = p.neighbours && V > 1 ? 2 * p.pairs / V : p.pairs / V;
     const int per_token = p.chunks * (p.heads[0] + p.heads[1]);
-    for (int e = threadIdx.x; e < n * per_token; e += ROT_THREADS) {
-        const int t = div_small(e, p.inv_items), r = e - t * per_token;
-        int head = div_small(r, p.inv_chunks);
-        const int c = r - head * p.chunks;
-        const int w = head >= p.heads[0];
-        head -= w ? p.heads[0] : 0;
-        const long long b = (first + t) / p.tokens, tok = first + t - b * p.tokens;
-        const T* x = (const T*)p.x[w] + b * p.xb[w] + tok * p.xt[w] + head * p.xh[w];
-        T* y = (T*)p.y[w] + b * p.yb[w] + tok * p.yt[w] + head * p.yh[w];
-        if (c >= turned) {  // behind the rotated dims
-            const int d = 2 * p.pairs + (c - turned) * V;
-            *(typename Vec<T, V>::type*)(y + d) = *(const typename Vec<T, V>::type*)(x + d);
-        } else if (!p.neighbours) {
-            const int i = c * V;
-            float u[V], v[V], uo[V], vo[V];
-            load_vec<T, V>(x + i, u);
-            load_vec<T, V>(x + i + p.pairs, v);
+    const int all_items = n * per_token;
+    typedef typename Vec<T, V>::type vec;
+    // ROT_AHEAD items a thread at a time, their loads issued before the first is used
+    for (int e0 = threadIdx.x; e0 < all_items; e0 += ROT_THREADS * ROT_AHEAD) {
+        vec u[ROT_AHEAD], v[ROT_AHEAD];
+        T* y[ROT_AHEAD];
+        int c[ROT_AHEAD], angle[ROT_AHEAD];  // c < 0: no item
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float cj = cs[t * p.pairs + i + j], sj = sn[t * p.pairs + i + j];
-                uo[j] = u[j] * cj - v[j] * sj;
-                vo[j] = v[j] * cj + u[j] * sj;
+        for (int k = 0; k < ROT_AHEAD; ++k) {
+            const int e = e0 + k * ROT_THREADS;
+            c[k] = -1;
+            if (e >= all_items) continue;
+            const int t = div_small(e, p.inv_items), r = e - t * per_token;
+            int head = div_small(r, p.inv_chunks);
+            c[k] = r - head * p.chunks;
+            angle[k] = t * p.pairs;
+            const int w = head >= p.heads[0];
+            head -= w ? p.heads[0] : 0;
+            const T* x = (const T*)p.x[w] + at[w][t] + head * p.xh[w];
+            y[k] = (T*)p.y[w] + at[2 + w][t] + head * p.yh[w];
+            if (V == 1 && p.neighbours && c[k] < turned) {
+                u[k] = *(const vec*)(x + 2 * c[k]);
+                v[k] = *(const vec*)(x + 2 * c[k] + 1);
+            } else {
+                const int d = c[k] < turned ? c[k] * V : 2 * p.pairs + (c[k] - turned) * V;
+                u[k] = *(const vec*)(x + d);
+                if (!p.neighbours && c[k] < turned) v[k] = *(const vec*)(x + d + p.pairs);
             }
-            store_vec<T, V>(y + i, uo);
-            store_vec<T, V>(y + i + p.pairs, vo);
-        } else if constexpr (V > 1) {
-            const int d = c * V;
-            float u[V], o[V];
-            load_vec<T, V>(x + d, u);
+        }
 #pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                const float cj = cs[t * p.pairs + (d + j) / 2], sj = sn[t * p.pairs + (d + j) / 2];
-                o[j] = u[j] * cj - u[j + 1] * sj;
-                o[j + 1] = u[j + 1] * cj + u[j] * sj;
+        for (int k = 0; k < ROT_AHEAD; ++k) {
+            if (c[k] < 0) continue;
+            if (c[k] >= turned) {  // behind the rotated dims
+                *(vec*)(y[k] + 2 * p.pairs + (c[k] - turned) * V) = u[k];
+            } else if (!p.neighbours || V == 1) {
+                const int i = c[k] * V;
+                float uo[V], vo[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float a, b;
+                    if constexpr (V == 1)
+                        a = (float)u[k], b = (float)v[k];
+                    else
+                        a = (float)u[k][j], b = (float)v[k][j];
+                    const float cj = cs[angle[k] + i + j], sj = sn[angle[k] + i + j];
+                    uo[j] = a * cj - b * sj;
+                    vo[j] = b * cj + a * sj;
+                }
+                store_vec<T, V>(y[k] + (V == 1 && p.neighbours ? 2 * i : i), uo);
+                store_vec<T, V>(y[k] + (V == 1 && p.neighbours ? 2 * i + 1 : i + p.pairs), vo);
+            } else if constexpr (V > 1) {
+                const int d = c[k] * V;
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    const float a = (float)u[k][j], b = (float)u[k][j + 1];
+                    const float cj = cs[angle[k] + (d + j) / 2], sj = sn[angle[k] + (d + j) / 2];
+                    o[j] = a * cj - b * sj;
+                    o[j + 1] = b * cj + a * sj;
+                }
+                store_vec<T, V>(y[k] + d, o);
             }
-            store_vec<T, V>(y + d, o);
-        } else {
-            const float u = (float)x[2 * c], v = (float)x[2 * c + 1], cj = cs[t * p.pairs + c], sj = sn[t * p.pairs + c];
-            y[2 * c] = (T)(u * cj - v * sj);
-            y[2 * c + 1] = (T)(v * cj + u * sj);
         }
     }
 }

@@ -243,26 +243,31 @@ AttnPlan attn_plan(const hat_attention* a)
     AttnPlan p{};
     const int group = a->q_heads / a->kv_heads;
     const long long rows = a->q_tokens * group;
-    p.split = !a->cu_q && rows <= 64;
-    if (p.split) {
-        p.tiles = (int)((rows + 31) / 32);
-        // Enough chunks that every CU has two blocks, of 256 keys at least.
-        const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
-        const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
-        p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / 512 + 127) / 128 * 128));
-        const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
-        const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
-        p.slots = (int)(a->cu_k ? slots : std::max<long long>(n, 1));
-        p.blocks = slots * a->kv_heads * p.tiles;
-        if (n > 1) {
-            p.join_rows = rows * a->kv_heads * a->n_seq;
-            p.workspace = (size_t)(slots * a->kv_heads * rows) * (a->head_dim + 2) * sizeof(float);
-        }
-    } else {
-        const int per = dim_tiles(a) <= 2 && a->dtype != HAT_F32 ? 256 : 128;  // rows a block (SEQ_INST)
-        const long long tiles = a->cu_q ? rows / per + a->n_seq : (rows + per - 1) / per;
-        p.blocks = tiles * a->kv_heads * (a->cu_q ? 1 : a->n_seq);
-        p.tiles = (int)tiles;
+    const auto tiles = [&](int per) { return a->cu_q ? rows / per + a->n_seq : (rows + per - 1) / per; };
+    const long long pairs = (long long)a->kv_heads * (a->cu_q ? 1 : a->n_seq);
+    p.tiles = (int)tiles(128);
+    p.blocks = tiles(128) * pairs;
+    // Few rows a sequence, or too few tiles of 128 to give half the CUs a block: tiles of
+    // 32 whose keys the waves (and blocks) share. Times at rows.. see attnseq.hip.
+    p.split = (!a->cu_q && rows <= 64) || p.blocks < 128;
+    if (!p.split) return p;
+    p.tiles = (int)tiles(32);
+    if (a->cu_q) {
+        p.blocks = tiles(32) * a->kv_heads;
+        p.chunk = 1 << 30;
+        return p;
+    }
+    // Enough chunks that every CU has two blocks, of 256 keys at least.
+    const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
+    const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
+    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / 512 + 127) / 128 * 128));
+    const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
+    const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
+    p.slots = (int)(a->cu_k ? slots : std::max<long long>(n, 1));
+    p.blocks = slots * a->kv_heads * p.tiles;
+    if (n > 1) {
+        p.join_rows = rows * a->kv_heads * a->n_seq;
+        p.workspace = (size_t)(slots * a->kv_heads * rows) * (a->head_dim + 2) * sizeof(float);
     }
     return p;
 }
@@ -339,10 +344,15 @@ void op_attention(const hat_attention* a, void* stream)
     hipStream_t s = check_stream(op, stream);
     const std::string type = type_name(a->dtype);
     std::string name = "hat_attnseq_" + type + "_d" + std::to_string(dim_tiles(a));
+    // The bias as MFMA's starting value needs it in units of q . k: not where the scale is
+    // next to nothing. fp32 has no kernel for the cap alone: its tanh is computed in full.
     if (plan.split)
         name += "_split";
-    else if (a->dtype != HAT_F32 && (a->cap > 0.0f || a->slopes))
-        name += "_gen";
+    else if (a->cap > 0.0f)
+        name += a->slopes || a->dtype == HAT_F32 ? "_both" : "_cap";
+    else if (a->slopes)
+        name += p.c1 > 1e-6f ? "_bias" : "_both";
+    p.fold = p.causal && !a->cu_q && plan.blocks <= 1024;
     const int threads = plan.split && a->dtype == HAT_F32 && dim_tiles(a) > 2 ? 128 : 256;
     launch(s, name.c_str(), grid_of(op, plan.blocks), 1, 1, threads, p);
     if (plan.join_rows)
@@ -380,14 +390,15 @@ void op_residual_norm(const hat_residual_norm* a, void* stream)
                 {"x_out", a->x_out, a->x_out_stride, true},
                 {"h", a->h, a->h_stride, true}};
     if (!a->x) throw Error("residual_norm: x is null");
-    bool wide = a->width % (16 / (int)e) == 0;
+    size_t move = 16;  // bytes a move: 16, 4 or one element
+    while ((size_t)a->width * e % move) move /= 4;
     for (const auto& r : rows) {
         if (!r.p) continue;
         check_pointer(op, r.what, r.p, e);
         check_stride(op, r.what, r.stride);
         if (r.out && a->rows > 1 && r.stride < a->width)
             throw Error(std::string("residual_norm: ") + r.what + " has rows on top of one another");
-        wide = wide && ((uintptr_t)r.p | (size_t)r.stride * e) % 16 == 0;
+        while (((uintptr_t)r.p | (size_t)r.stride * e) % move) move /= 4;
     }
     for (int i = 0; i < 2; ++i)
         for (int o = 3; o < 5; ++o)
@@ -397,7 +408,7 @@ void op_residual_norm(const hat_residual_norm* a, void* stream)
     for (const float* w : {a->post_w, a->post_b, a->pre_w, a->pre_b}) {
         if (!w) continue;
         check_pointer(op, "a norm's weight", w, 4);
-        wide = wide && (uintptr_t)w % 16 == 0;
+        if ((uintptr_t)w % 16 && move == 16) move = 4;
     }
     ResNormArgs p{};
     p.x = a->x, p.y = a->y, p.gate = a->gate, p.xo = a->x_out, p.h = a->h;
@@ -410,8 +421,8 @@ void op_residual_norm(const hat_residual_norm* a, void* stream)
     const int W = a->width;
     const char* form;
     int per, threads = 256;
-    if (!wide)
-        form = W <= 1024 ? "64e" : "1024e", per = W <= 1024 ? 4 : 1;
+    if (move < 16)
+        form = move > e ? (W <= 1024 ? "64h" : "1024h") : W <= 1024 ? "64e" : "1024e", per = W <= 1024 ? 4 : 1;
     else if (W <= (a->dtype == HAT_F32 ? 192 : 256))
         form = "16", per = 16;
     else if (W <= (a->dtype == HAT_F32 ? 1024 : 2048))

@@ -10,6 +10,7 @@ device is missing.
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -132,10 +133,11 @@ def lib():
                                    _f32p, _f32p, _f32p, _f32p, _f32p, C.c_int, _f32p, _f32p]),
         "hat_op_ocab": (C.c_int, [_f32p, _f32p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]
                         + [_f32p] * 13 + [C.c_int, _f32p, _f32p]),
-        "hat_op_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
-        "hat_op_attention_workspace": (C.c_size_t, [C.POINTER(AttentionArgs)]),
-        "hat_op_attention": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
-        "hat_op_residual_norm": (C.c_int, [C.POINTER(ResidualNormArgs), C.c_void_p]),
+        # structures: by reference, or packed bytes
+        "hat_op_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
+        "hat_op_attention_workspace": (C.c_size_t, [C.c_void_p]),
+        "hat_op_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+        "hat_op_residual_norm": (C.c_int, [C.c_void_p, C.c_void_p]),
         "hat_device_alloc": (C.c_void_p, [C.c_size_t]),
         "hat_device_free": (C.c_int, [C.c_void_p]),
         "hat_memcpy_h2d": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
@@ -549,39 +551,72 @@ def _code(t, what):
     return c
 
 
+_fns = {}
+
+
+def _fn(name):
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(lib(), name)
+    return f
+
+
+def _packed(op, layout, *fields):
+    try:
+        return layout.pack(*fields)
+    except (struct.error, OverflowError) as e:  # a size or a factor that its field cannot hold
+        raise HatError(f"{op}: an argument is out of range ({e})")
+
+
+# The argument structures packed in one go, field by field as they are declared above
+# (a ctypes structure costs a call an assignment a field).
+_ROTARY = struct.Struct("@6iq4i3id4q16q")
+_ATTENTION = struct.Struct("@6i2q16q5QifffQ8qQQ")
+_NORM = struct.Struct("@4i2q5Q5q4Q3f4x")
+_NO_HEADS = (0, 0, 0, 0)
+
+
 def _heads(t, what, code, lead=None):
-    """(Heads, batch, tokens, heads, dim) of [batch, token, head, dim] or [token, head, dim]."""
+    """(the fields of Heads, batch, tokens, heads, dim) of [batch, token, head, dim] or
+    [token, head, dim]."""
     if _code(t, what) != code:
         raise HatError(f"{what}: type {t.dtype} differs from the first tensor's")
     shape, st = t.shape, t.stride()
-    if len(shape) not in (3, 4):
+    if lead is not None and shape != lead:
+        raise HatError(f"{what}: {tuple(shape)} where {tuple(lead)} is expected")
+    n = len(shape)
+    if n == 4:
+        batch, tokens, heads, dim = shape
+        fields = (t.data_ptr(), st[0], st[1], st[2])
+    elif n == 3:
+        tokens, heads, dim = shape
+        batch, fields = 1, (t.data_ptr(), 0, st[0], st[1])
+    else:
         raise HatError(f"{what}: [batch, token, head, dim] or [token, head, dim] expected, not {tuple(shape)}")
-    if shape[-1] > 1 and st[-1] != 1:
+    if st[-1] != 1 and dim > 1:
         raise HatError(f"{what}: the last axis must have stride 1")
-    if lead is not None and tuple(shape) != lead:
-        raise HatError(f"{what}: {tuple(shape)} where {lead} is expected")
-    if len(shape) == 4:
-        return Heads(t.data_ptr(), st[0], st[1], st[2]), shape[0], shape[1], shape[2], shape[3]
-    return Heads(t.data_ptr(), 0, st[0], st[1]), 1, shape[0], shape[1], shape[2]
+    return fields, batch, tokens, heads, dim
 
 
 def _positions(t, what, batch, tokens):
-    """(Positions, axes) of int32 [token, axis], shared by the batch, or [batch, token, axis]."""
+    """(the fields of Positions, axes) of int32 [token, axis], shared by the batch, or
+    [batch, token, axis]."""
     if _code(t, what) != 3:
         raise HatError(f"{what}: int32 expected, not {t.dtype}")
-    shape, st = tuple(t.shape), t.stride()
+    shape, st = t.shape, t.stride()
     if len(shape) == 2 and shape[0] == tokens:
-        return Positions(t.data_ptr(), 0, st[0], st[1]), shape[1]
-    if len(shape) == 3 and shape[:2] == (batch, tokens):
-        return Positions(t.data_ptr(), st[0], st[1], st[2]), shape[2]
-    raise HatError(f"{what}: {shape} is no [{tokens}, axis] or [{batch}, {tokens}, axis]")
+        return (t.data_ptr(), 0, st[0], st[1]), shape[1]
+    if len(shape) == 3 and shape[0] == batch and shape[1] == tokens:
+        return (t.data_ptr(), st[0], st[1], st[2]), shape[2]
+    raise HatError(f"{what}: {tuple(shape)} is no [{tokens}, axis] or [{batch}, {tokens}, axis]")
 
 
 def _vector(t, what, code, n):
-    """The pointer of a contiguous vector of n values, or None."""
+    """The pointer of a contiguous vector of n values, or 0."""
     if t is None:
-        return None
-    if _code(t, what) != code or tuple(t.shape) != (n,) or (n > 1 and t.stride()[0] != 1):
+        return 0
+    shape = t.shape
+    if _code(t, what) != code or len(shape) != 1 or shape[0] != n or (n > 1 and t.stride()[0] != 1):
         raise HatError(f"{what}: {n} contiguous values of {'fp32' if code == 0 else 'int32'} expected")
     return t.data_ptr()
 
@@ -591,27 +626,25 @@ def op_rotary(q, k, pos, sections, base=10000.0, pairs="halves", joint=False, in
     """hat_op_rotary: turns q and k (None: q alone) by their tokens' positions, in place
     where q_out / k_out are left out. pairs: "halves" or "neighbours"; stream: a
     hipStream_t as an integer (torch's `cuda_stream`), None the default stream."""
-    a = RotaryArgs()
-    a.dtype = code = _code(q, "rotary: q")
-    a.q, a.batch, a.tokens, a.q_heads, a.head_dim = _heads(q, "rotary: q", code)
-    a.q_out = a.q if q_out is None else _heads(q_out, "rotary: q_out", code, tuple(q.shape))[0]
+    code = _code(q, "rotary: q")
+    fq, batch, tokens, q_heads, dim = _heads(q, "rotary: q", code)
+    fqo = fq if q_out is None else _heads(q_out, "rotary: q_out", code, q.shape)[0]
+    k_heads, fk, fko = 0, _NO_HEADS, _NO_HEADS
     if k is not None:
-        a.k, b, t, a.k_heads, d = _heads(k, "rotary: k", code)
-        if (b, t, d) != (a.batch, a.tokens, a.head_dim):
+        fk, b, t, k_heads, d = _heads(k, "rotary: k", code)
+        if b != batch or t != tokens or d != dim:
             raise HatError(f"rotary: k of {tuple(k.shape)} does not go with q of {tuple(q.shape)}")
-        a.k_out = a.k if k_out is None else _heads(k_out, "rotary: k_out", code, tuple(k.shape))[0]
+        fko = fk if k_out is None else _heads(k_out, "rotary: k_out", code, k.shape)[0]
     elif k_out is not None:
         raise HatError("rotary: k_out without k")
-    a.pos, axes = _positions(pos, "rotary: pos", a.batch, a.tokens)
+    fp, axes = _positions(pos, "rotary: pos", batch, tokens)
     if axes != len(sections) or not 1 <= axes <= 4:
         raise HatError(f"rotary: {axes} axes of positions and {len(sections)} sections (1 to 4)")
     if pairs not in ("halves", "neighbours"):
         raise HatError(f"rotary: pairs are halves or neighbours, not {pairs!r}")
-    a.axes = axes
-    for i, n in enumerate(sections):
-        a.sections[i] = n
-    a.joint, a.neighbours, a.inverse, a.base = bool(joint), pairs == "neighbours", bool(inverse), base
-    _check(lib().hat_op_rotary(C.byref(a), stream), "rotary")
+    _check(_fn("hat_op_rotary")(_packed("rotary", _ROTARY, code, batch, q_heads, k_heads, dim, axes, tokens,
+                                        *sections, *(0,) * (4 - axes), bool(joint), pairs == "neighbours",
+                                        bool(inverse), base, *fp, *fq, *fqo, *fk, *fko), stream), "rotary")
 
 
 def _sequences(cu, what):
@@ -620,52 +653,47 @@ def _sequences(cu, what):
     return cu.shape[0] - 1
 
 
-def _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k):
-    a = AttentionArgs()
-    a.dtype = code = _code(q, "attention: q")
-    a.q, bq, a.q_tokens, a.q_heads, a.head_dim = _heads(q, "attention: q", code)
-    a.k, bk, a.k_tokens, a.kv_heads, d = _heads(k, "attention: k", code)
-    a.v = _heads(v, "attention: v", code, tuple(k.shape))[0]
-    a.out = _heads(out, "attention: out", code, tuple(q.shape))[0]
-    if d != a.head_dim:
-        raise HatError(f"attention: head_dim {a.head_dim} of q and {d} of k")
-    n = _sequences(cu_q, "attention: cu_q") if cu_q is not None else None
-    if cu_k is not None:
-        m = _sequences(cu_k, "attention: cu_k")
-        if n is not None and m != n:
-            raise HatError(f"attention: {n} sequences in cu_q and {m} in cu_k")
-        n = m
-    if n is None:
-        n = bq
-    if (cu_q is not None and len(q.shape) != 3) or (cu_k is not None and len(k.shape) != 3):
-        raise HatError("attention: a packed tensor is [token, head, dim]")
+def _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k,
+                    workspace=0, workspace_bytes=0):
+    code = _code(q, "attention: q")
+    fq, bq, q_tokens, q_heads, dim = _heads(q, "attention: q", code)
+    fk, bk, k_tokens, kv_heads, d = _heads(k, "attention: k", code)
+    fv = _heads(v, "attention: v", code, k.shape)[0]
+    fo = _heads(out, "attention: out", code, q.shape)[0]
+    if d != dim:
+        raise HatError(f"attention: head_dim {dim} of q and {d} of k")
+    n = bq
+    if cu_q is not None or cu_k is not None:
+        n = _sequences(cu_q, "attention: cu_q") if cu_q is not None else None
+        if cu_k is not None:
+            m = _sequences(cu_k, "attention: cu_k")
+            if n is not None and m != n:
+                raise HatError(f"attention: {n} sequences in cu_q and {m} in cu_k")
+            n = m
+        if (cu_q is not None and len(q.shape) != 3) or (cu_k is not None and len(k.shape) != 3):
+            raise HatError("attention: a packed tensor is [token, head, dim]")
     if (cu_q is None and bq != n) or (cu_k is None and bk != n):
         raise HatError(f"attention: q of {tuple(q.shape)} and k of {tuple(k.shape)} are not {n} sequences")
-    a.n_seq = n
-    a.cu_q = _vector(cu_q, "attention: cu_q", 3, n + 1)
-    a.cu_k = _vector(cu_k, "attention: cu_k", 3, n + 1)
-    a.q_lens = _vector(q_lens, "attention: q_lens", 3, n)
-    a.k_lens = _vector(k_lens, "attention: k_lens", 3, n)
-    a.prefix = _vector(prefix, "attention: prefix", 3, n)
-    a.slopes = _vector(slopes, "attention: slopes", 0, a.q_heads)
-    a.causal = bool(causal)
-    a.scale = a.head_dim ** -0.5 if scale is None else scale
-    a.cap = cap
+    axes, fpq, fpk = 0, _NO_HEADS, _NO_HEADS
     if pos_q is not None and pos_k is not None:
-        a.pos_q, a.axes = _positions(pos_q, "attention: pos_q", bq, a.q_tokens)
-        a.pos_k, axes = _positions(pos_k, "attention: pos_k", bk, a.k_tokens)
-        if axes != a.axes:
-            raise HatError(f"attention: {a.axes} axes in pos_q and {axes} in pos_k")
+        fpq, axes = _positions(pos_q, "attention: pos_q", bq, q_tokens)
+        fpk, d = _positions(pos_k, "attention: pos_k", bk, k_tokens)
+        if d != axes:
+            raise HatError(f"attention: {axes} axes in pos_q and {d} in pos_k")
     elif pos_q is not None or pos_k is not None:
         raise HatError("attention: positions of queries and keys go together")
-    return a
+    return _packed("attention", _ATTENTION, code, n, q_heads, kv_heads, dim, axes, q_tokens, k_tokens, *fq, *fk, *fv,
+                   *fo, _vector(cu_q, "attention: cu_q", 3, n + 1), _vector(cu_k, "attention: cu_k", 3, n + 1),
+                   _vector(q_lens, "attention: q_lens", 3, n), _vector(k_lens, "attention: k_lens", 3, n),
+                   _vector(prefix, "attention: prefix", 3, n), bool(causal), dim ** -0.5 if scale is None else scale,
+                   cap, 0.0, _vector(slopes, "attention: slopes", 0, q_heads), *fpq, *fpk, workspace, workspace_bytes)
 
 
 def attention_workspace(q, k, v, out, scale=None, causal=False, prefix=None, cu_q=None, cu_k=None, q_lens=None,
                         k_lens=None, cap=0.0, slopes=None, pos_q=None, pos_k=None):
     """The bytes that op_attention of these arguments needs as its workspace."""
-    a = _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k)
-    n = lib().hat_op_attention_workspace(C.byref(a))
+    n = _fn("hat_op_attention_workspace")(_attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens,
+                                                          k_lens, cap, slopes, pos_q, pos_k))
     if n == C.c_size_t(-1).value:
         raise HatError(f"attention: {_err()}")
     return n
@@ -676,21 +704,23 @@ def op_attention(q, k, v, out, scale=None, causal=False, prefix=None, cu_q=None,
     """hat_op_attention: [batch, token, head, dim] tensors, or packed [token, head, dim] with
     cu_q / cu_k; scale None: head_dim^-1/2; workspace: a device tensor of at least
     attention_workspace(...) bytes where that is not 0; stream as op_rotary's."""
-    a = _attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap, slopes, pos_q, pos_k)
+    ptr = size = 0
     if workspace is not None:
         size = _SIZES[_code(workspace, "attention: workspace")]
         if len(workspace.shape) != 1 or (workspace.shape[0] > 1 and workspace.stride()[0] != 1):
             raise HatError("attention: the workspace is one contiguous row")
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.shape[0] * size
-    _check(lib().hat_op_attention(C.byref(a), stream), "attention")
+        ptr, size = workspace.data_ptr(), workspace.shape[0] * size
+    _check(_fn("hat_op_attention")(_attention_args(q, k, v, out, scale, causal, prefix, cu_q, cu_k, q_lens, k_lens, cap,
+                                                   slopes, pos_q, pos_k, ptr, size), stream), "attention")
 
 
 def _rows(t, what, code, lead=None):
+    """(pointer, row stride) of [rows, width]."""
     if _code(t, what) != code:
         raise HatError(f"{what}: type {t.dtype} differs from x's")
-    shape, st = tuple(t.shape), t.stride()
-    if len(shape) != 2 or (shape[1] > 1 and st[1] != 1) or (lead is not None and shape != lead):
-        raise HatError(f"{what}: {shape} is no [rows, width] of stride 1" + (f" like x's {lead}" if lead else ""))
+    shape, st = t.shape, t.stride()
+    if len(shape) != 2 or (st[1] != 1 and shape[1] > 1) or (lead is not None and shape != lead):
+        raise HatError(f"{what}: {tuple(shape)} is no [rows, width] of stride 1" + (f" like x's {tuple(lead)}" if lead else ""))
     return t.data_ptr(), st[0]
 
 
@@ -700,31 +730,32 @@ def op_residual_norm(x, y=None, x_out=None, h=None, gate=None, scale=1.0, post="
     """hat_op_residual_norm on [rows, width] tensors: x_out = x + scale * gate * N(y), h =
     N(x_out), either left out where None. gate: [gates, width], a row for each rows / gates
     rows; post, pre: "none", "layer" or "rms" with fp32 weights; post_eps None: eps."""
-    a = ResidualNormArgs()
-    a.dtype = code = _code(x, "residual_norm: x")
+    code = _code(x, "residual_norm: x")
     if code > 2:
         raise HatError(f"residual_norm: type {x.dtype} is not supported")
-    a.x, a.x_stride = _rows(x, "residual_norm: x", code)
-    lead = tuple(x.shape)
-    a.rows, a.width = lead
+    px, sx = _rows(x, "residual_norm: x", code)
+    lead = x.shape
+    rows, width = lead
+    py = sy = pxo = sxo = ph = sh = pg = sg = 0
+    per = 1
     if y is not None:
-        a.y, a.y_stride = _rows(y, "residual_norm: y", code, lead)
+        py, sy = _rows(y, "residual_norm: y", code, lead)
     if x_out is not None:
-        a.x_out, a.x_out_stride = _rows(x_out, "residual_norm: x_out", code, lead)
+        pxo, sxo = _rows(x_out, "residual_norm: x_out", code, lead)
     if h is not None:
-        a.h, a.h_stride = _rows(h, "residual_norm: h", code, lead)
+        ph, sh = _rows(h, "residual_norm: h", code, lead)
     if gate is not None:
-        a.gate, a.gate_stride = _rows(gate, "residual_norm: gate", code)
+        pg, sg = _rows(gate, "residual_norm: gate", code)
         n = gate.shape[0]
-        if gate.shape[1] != a.width or n < 1 or a.rows % n:
-            raise HatError(f"residual_norm: gates of {tuple(gate.shape)} for x of {lead}")
-        a.rows_per_gate = max(1, a.rows // n)
+        if gate.shape[1] != width or n < 1 or rows % n:
+            raise HatError(f"residual_norm: gates of {tuple(gate.shape)} for x of {tuple(lead)}")
+        per = max(1, rows // n)
     if post not in _NORMS or pre not in _NORMS:
         raise HatError(f"residual_norm: norms are none, layer or rms, not {post!r}, {pre!r}")
-    a.post, a.pre = _NORMS[post], _NORMS[pre]
-    a.post_w = _vector(post_weight, "residual_norm: post_weight", 0, a.width)
-    a.post_b = _vector(post_bias, "residual_norm: post_bias", 0, a.width)
-    a.pre_w = _vector(pre_weight, "residual_norm: pre_weight", 0, a.width)
-    a.pre_b = _vector(pre_bias, "residual_norm: pre_bias", 0, a.width)
-    a.scale, a.pre_eps, a.post_eps = scale, eps, eps if post_eps is None else post_eps
-    _check(lib().hat_op_residual_norm(C.byref(a), stream), "residual_norm")
+    _check(_fn("hat_op_residual_norm")(_packed(
+        "residual_norm", _NORM, code, width, _NORMS[post], _NORMS[pre], rows, per, px, py, pg, pxo, ph, sx, sy, sg, sxo, sh,
+        _vector(post_weight, "residual_norm: post_weight", 0, width),
+        _vector(post_bias, "residual_norm: post_bias", 0, width),
+        _vector(pre_weight, "residual_norm: pre_weight", 0, width),
+        _vector(pre_bias, "residual_norm: pre_bias", 0, width), scale, eps if post_eps is None else post_eps, eps),
+        stream), "residual_norm")

@@ -172,3 +172,30 @@ def test_structures_are_the_header_s():
     for t in names.values():
         want += [ctypes.sizeof(t)] + [getattr(t, f[0]).offset for f in t._fields_]
     assert got == want
+
+
+def test_packed_layouts_are_the_structures():
+    """The layouts that calls pack against the structures of the same fields."""
+    def leaves(t, path=()):
+        for name, kind in t._fields_:
+            if hasattr(kind, "_fields_"):
+                yield from leaves(kind, path + (name,))
+            elif hasattr(kind, "_length_"):
+                yield from ((path + (name, i), kind._type_) for i in range(kind._length_))
+            else:
+                yield path + (name,), kind
+
+    for layout, t in ((hl._ROTARY, hl.RotaryArgs), (hl._ATTENTION, hl.AttentionArgs), (hl._NORM, hl.ResidualNormArgs)):
+        a, values = t(), []
+        for n, (path, kind) in enumerate(leaves(t), 1):
+            to = a
+            for step in path[:-1]:
+                to = getattr(to, step) if isinstance(step, str) else to[step]
+            if isinstance(path[-1], str):
+                setattr(to, path[-1], n)
+            else:
+                to[path[-1]] = n
+            values.append(n)
+        if t is hl.AttentionArgs:  # the gap between cap and slopes is a field of the layout
+            values.insert(values.index([i for i, (p, _) in enumerate(leaves(t), 1) if p == ("slopes",)][0]), 0.0)
+        assert layout.pack(*values) == bytes(a)
