@@ -286,16 +286,18 @@ def _attention_want(q, k, v, seqs, scale, causal, prefix, cap, slopes, pos_q, po
     """(want, tolerance) for rows of q [n, hq, D], keys of k [m, hk, D]; seqs: (q rows, k
     rows) slices of each sequence; rows of no sequence are NaN. sure: the type's U."""
     D, hq, hk = q.shape[-1], q.shape[1], k.shape[1]
-    want = torch.full(q.shape, math.nan, dtype=torch.float64)
-    tol = torch.zeros(q.shape, dtype=torch.float64)
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    prefix, slopes, pos_q, pos_k = (None if x is None else x.cuda() for x in (prefix, slopes, pos_q, pos_k))
+    want = torch.full(q.shape, math.nan, dtype=torch.float64, device="cuda")
+    tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     for n, (rq, rk) in enumerate(seqs):
         qs, ks, vs = q[rq].double(), k[rk].double(), v[rk].double()
         lq, lk = qs.shape[0], ks.shape[0]
         want[rq] = 0.0
         if lk == 0 or lq == 0:
             continue
-        i, j = torch.arange(lq)[:, None] + lk - lq, torch.arange(lk)[None]
-        hidden = torch.zeros(lq, lk, dtype=torch.bool)
+        i, j = torch.arange(lq, device="cuda")[:, None] + lk - lq, torch.arange(lk, device="cuda")[None]
+        hidden = torch.zeros(lq, lk, dtype=torch.bool, device="cuda")
         if causal:
             hidden = j > i
             if prefix is not None:
@@ -332,7 +334,7 @@ def _attention_want(q, k, v, seqs, scale, causal, prefix, cap, slopes, pos_q, po
             if sure == 2.0 ** -11:
                 t = t + 2.0 ** -24 * lk * vh.abs().max()
             tol[rq, h] = t + sure * 1.01 * (o.abs() + t)
-    return want, tol
+    return want.cpu(), tol.cpu()
 
 
 def _check(hl, kind, q, k, v, seqs, stride="plain", scale=None, causal=False, prefix=None, cap=0.0, slopes=None,
@@ -630,6 +632,124 @@ def test_attention_far_into_a_long_cache(hl):
                                 None, None, 2.0 ** -11)
     assert ((out[64].cpu().double() - want).abs() <= tol).all()
     assert (out[:64] == 0).all()  # sequences without keys
+
+
+# Enough sequences and key heads that tiles of 128 rows fill the device: the kernels of
+# many rows, each width of a head in each of their forms.
+
+MODES = {
+    "plain": dict(),
+    "index": dict(bias="index"),
+    "grid": dict(bias="grid"),
+    "cap": dict(cap=20.0),
+    "both": dict(cap=30.0, bias="index"),
+    "both grid": dict(cap=30.0, bias="grid"),
+    "no scale": dict(bias="index", scale=0.0),
+    "negative": dict(bias="index", scale=-0.2),
+}
+
+
+def _mode(mode, hq, lq, lk, B, seed):
+    more = dict(MODES[mode])
+    bias = more.pop("bias", None)
+    if bias:
+        more["slopes"] = torch.linspace(-0.02, 0.3, hq)
+    if bias == "grid":
+        g = _gen(seed)
+        more["pos_q"] = torch.randint(-20, 20, (lq, 3), generator=g, dtype=torch.int32)
+        more["pos_k"] = torch.randint(-20, 20, (lk, 3), generator=g, dtype=torch.int32)
+    return more
+
+
+@pytest.mark.parametrize("mode", list(MODES))
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [24, 64, 80, 128])
+def test_attention_many_tiles(hl, kind, D, mode):
+    B, lq, lk, hq, hk = 33, 75, 141, 8, 4
+    print(f"many tiles {kind} {D} {mode}", flush=True)
+    q, k, v = _qkv(kind, 201, (B, lq), (B, lk), hq, hk, D)
+    _check(hl, kind, q, k, v, _batch(B, lq, lk), causal=mode in ("index", "cap", "both"),
+           **_mode(mode, hq, lq, lk, B, 202))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [1, 30, 33, 72, 96, 127])
+@pytest.mark.parametrize("stride", ["plain", "odd", "heads"])
+def test_attention_many_tiles_of_odd_heads(hl, kind, D, stride):
+    B, lq, lk, hq, hk = 64, 129, 70, 2, 2
+    print(f"odd heads {kind} {D} {stride}", flush=True)
+    q, k, v = _qkv(kind, 211, (B, lq), (B, lk), hq, hk, D)
+    _check(hl, kind, q, k, v, _batch(B, lq, lk), stride=stride, causal=True, slopes=torch.tensor([0.1, 0.0]))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("mode", ["plain", "grid", "cap"])
+def test_attention_many_tiles_of_documents(hl, kind, mode):
+    """Packed documents of 0 to 300 tokens, more queries than keys in some."""
+    g = _gen(221)
+    lq, lk = torch.randint(0, 300, (40,), generator=g), torch.randint(0, 300, (40,), generator=g)
+    lq[3] = lk[5] = lq[39] = 0
+    cu_q, cu_k = (torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(torch.int32) for n in (lq, lk))
+    q, k, v = _qkv(kind, 222, (int(cu_q[-1]) + 7,), (int(cu_k[-1]) + 3,), 4, 2, 64)
+    print(f"many documents {kind} {mode}", flush=True)
+    _check(hl, kind, q, k, v, _packed(cu_q.tolist(), cu_k.tolist()), causal=True, cu_q=cu_q, cu_k=cu_k,
+           **_mode(mode, 4, q.shape[0], k.shape[0], 1, 223))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [32, 128])
+def test_attention_many_tiles_padded_with_a_prefix(hl, kind, D):
+    """Lengths of their own on both sides, prefixes, NaN and infinities behind the last
+    key and, in a prefix's tile, behind the prefix."""
+    B, lq, lk = 70, 140, 200
+    g = _gen(231)
+    uq, uk = (torch.randint(0, n + 1, (B,), generator=g) for n in (lq, lk))
+    prefix = torch.randint(0, 120, (B,), generator=g).to(torch.int32)
+    q, k, v = _qkv(kind, 232, (B, lq), (B, lk), 2, 2, D)
+    for b in range(B):
+        k[b, uk[b]:], v[b, uk[b]:] = math.nan, math.inf
+    _check(hl, kind, q, k, v, _batch(B, lq, lk, uq.tolist(), uk.tolist()), causal=True, prefix=prefix,
+           q_lens=uq.to(torch.int32), k_lens=uk.to(torch.int32))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_attention_many_tiles_unseen_keys_have_no_influence(hl, kind):
+    B, n, D = 64, 160, 64
+    q, k, v = _qkv(kind, 241, (B, n), (B, n), 2, 2, D)
+    kb, vb = k.clone(), v.clone()
+    kb[3, 70], vb[3, 70] = math.nan, math.inf
+    vb[9, 159] = math.nan
+    qd = q.cuda()
+    out, clean = torch.empty_like(qd), torch.empty_like(qd)
+    hl.op_attention(qd, kb.cuda(), vb.cuda(), out, causal=True)
+    hl.op_attention(qd, k.cuda(), v.cuda(), clean, causal=True)
+    torch.cuda.synchronize()
+    others = [b for b in range(B) if b not in (3, 9)]
+    assert torch.equal(out[others], clean[others])
+    assert out[3, 70:].isnan().all() and out[9, 159].isnan().all()
+    assert torch.isfinite(out[3, :70]).all() and torch.isfinite(out[9, :159]).all()
+    want, tol = _attention_want(q[3], k[3], v[3], [(slice(0, n), slice(0, n))], D ** -0.5, True, None, 0.0, None, None,
+                                None, U(q.dtype))
+    assert ((out[3].cpu().double() - want).abs()[:70] <= tol[:70]).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("mode", ["plain", "index"])
+def test_attention_many_tiles_score_spread(hl, kind, mode):
+    """The running maximum that moves at every stage, scores far apart and far from zero."""
+    for name in ("wide", "rising", "falling", "high", "flat"):
+        q, k, v = _qkv(kind, 251, (33, 70), (33, 400), 4, 4, 64)
+        if name == "wide":
+            q = (q.float() * 6).to(q.dtype)
+        elif name in ("rising", "falling"):
+            ramp = torch.linspace(0, 40, 400) if name == "rising" else torch.linspace(40, 0, 400)
+            q[..., 0], k[..., 0] = 8.0, ramp[None, :, None].to(k.dtype)
+        elif name == "high":
+            q[..., 0], k[..., 0] = 30.0, 30.0
+        else:
+            q.zero_()
+        print(f"many tiles spread {kind} {mode} {name}", flush=True)
+        _check(hl, kind, q, k, v, _batch(33, 70, 400), **_mode(mode, 4, 70, 400, 33, 0))
 
 
 # ---- together ------------------------------------------------------------------------
