@@ -274,6 +274,32 @@ __device__ __forceinline__ void load_q(const SeqAttnArgs& p, const SeqView& v, c
     }
 }
 
+// The same from fp32, split: eight dims a step and lane half.
+template <int DT>
+__device__ __forceinline__ void load_q32(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r, u32x4 (&q)[2 * DT][3])
+{
+    const int h = (threadIdx.x >> 5) & 1;
+    const float* row = (const float*)p.q + v.bq * p.qb + (long long)(v.q0 + r.i) * p.qt + r.head * p.qh;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+    for (int ks = 0; ks < 2 * DT; ++ks) {
+        float f[8];
+#pragma unroll
+        for (int x = 0; x < 8; x += 4) {
+            const int d0 = (2 * ks + h) * 8 + x;
+            if (p.wide) {
+                const f32x4 u = r.live && d0 < p.dim ? *(const f32x4*)(row + d0) : (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[x + e] = u[e] * sign;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[x + e] = r.live && d0 + e < p.dim ? row[d0 + e] * sign : 0.0f;
+            }
+        }
+        split3_x8(f, q[ks]);
+    }
+}
+
 // One lane's running softmax over the keys of its row.
 template <class T, int DT>
 struct SeqAcc {
@@ -519,6 +545,18 @@ __device__ __forceinline__ void seq_exp(const SeqAttnArgs& p, f32x16 (&s)[QT][KT
     }
 }
 
+// V's 16-bit operand of one MFMA: two transposed reads, four keys each, `step` bytes apart.
+__device__ __forceinline__ u32x4 read_v(const unsigned char* at, int step)
+{
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const u2 a = __builtin_bit_cast(
+        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+    const u2 b = __builtin_bit_cast(
+        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + step)));
+    return (u32x4){a[0], a[1], b[0], b[1]};
+}
+
 // O^T += V^T P^T. With MFMA's key order within 16 (lane half h, slot j: keys 4 h + j,
 // then 8 + 4 h + j - 4) V's 16-bit operand is two transposed reads of four keys each.
 template <class T, int DT, int QT, int KT>
@@ -541,7 +579,6 @@ __device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)
                 }
             }
     } else {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
         const int x = lane & 15, kr = 4 * h + (x >> 2);
         const int row = kr * S::ROW + (x & 1) * 8;
         const int lc = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1), vsw = S::vswz(kr);
@@ -551,15 +588,10 @@ __device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const unsigned char* at = V + row + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4*)(at + 8 * S::ROW));
-                    typedef unsigned u2 __attribute__((ext_vector_type(2)));
-                    const u2 a = __builtin_bit_cast(u2, lo), b = __builtin_bit_cast(u2, hi);
+                    const u32x4 a = read_v(V + row + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW, 8 * S::ROW);
 #pragma unroll
                     for (int t = 0; t < QT; ++t)
-                        acc[t].o[d] = mma16((u32x4){a[0], a[1], b[0], b[1]}, pb[t][kt][st], acc[t].o[d], T());
+                        acc[t].o[d] = mma16(a, pb[t][kt][st], acc[t].o[d], T());
                 }
     }
 }
@@ -610,31 +642,38 @@ __device__ __forceinline__ SeqView uniform(const SeqView& v)
     return w;
 }
 
-// ---- many rows: a block of four waves, QT x 32 rows each, walks the keys in stages of
-// KT x 32, two in LDS: the next one's copy runs under the present one's products.
-template <class T, int DT, int QT, int KT, int MODE>
-__device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0, unsigned char* K1, unsigned char* V0,
-                                         unsigned char* V1, unsigned* P0, unsigned* P1)
+// A block's tile of 128 QT rows, and its waves' shares: 32 QT rows each.
+struct SeqTile {
+    SeqView v;
+    int kvh, rows, prefix;
+    int row0;         // the wave's first row
+    int end;          // the block's keys
+    int least, most;  // the least and the largest limit of the wave's rows (limits rise with the row)
+    int at0, at1;     // i + Lk - Lq of its first and last row
+};
+
+template <int QT>
+__device__ __forceinline__ bool seq_tile(const SeqAttnArgs& p, SeqTile& w)
 {
-    constexpr int BQ = 128 * QT, BK = 32 * KT;
+    constexpr int BQ = 128 * QT;
     const int pairs = p.cu_q ? p.kv_heads : p.kv_heads * p.n_seq;
     const int pair = blockIdx.x % pairs;
-    int tile = blockIdx.x / pairs, sq, kvh;
+    int tile = blockIdx.x / pairs, sq;
     if (p.cu_q) {
         int first = 0;
-        kvh = pair;
+        w.kvh = pair;
         sq = find_sequence(p.cu_q, p.n_seq, p.q_tokens, p.group, BQ, tile, first);
-        if (sq < 0) return;
+        if (sq < 0) return false;
         tile -= first;
     } else {
         sq = pair / p.kv_heads;
-        kvh = pair - sq * p.kv_heads;
+        w.kvh = pair - sq * p.kv_heads;
     }
-    const SeqView v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
+    const SeqView v = w.v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
     tile = __builtin_amdgcn_readfirstlane(tile);
-    const int rows = v.lq * p.group;
-    const int tiles = (rows + BQ - 1) / BQ;
-    if (tile >= tiles) return;
+    w.rows = v.lq * p.group;
+    const int tiles = (w.rows + BQ - 1) / BQ;
+    if (tile >= tiles) return false;
     // Under the causal mask a tile's work grows with its number: the longest first, and
     // where all blocks run at once (p.fold) the second half from the shortest on, so that
     // the CUs, which take blocks in turn, get a long and a short one each.
@@ -642,12 +681,78 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
         const int half = (tiles + 1) / 2;
         tile = p.fold && tile >= half ? tile - half : tiles - 1 - tile;
     }
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
-    const int row0 = tile * BQ + wave * 32 * QT;
-    const int row_last = tile * BQ + BQ - 1 < rows ? tile * BQ + BQ - 1 : rows - 1;
-    const int end = row_limit(p, v, row_last / p.group, prefix);
+    w.prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
+    w.row0 = tile * BQ + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32 * QT;
+    const int block_last = tile * BQ + BQ - 1 < w.rows ? tile * BQ + BQ - 1 : w.rows - 1;
+    w.end = row_limit(p, v, block_last / p.group, w.prefix);
+    w.least = 0x7fffffff, w.most = 0;
+    if (w.row0 < w.rows) {
+        w.least = row_limit(p, v, w.row0 / p.group, w.prefix);
+        const int last = w.row0 + 32 * QT - 1 < w.rows ? w.row0 + 32 * QT - 1 : w.rows - 1;
+        w.most = row_limit(p, v, last / p.group, w.prefix);
+    }
+    w.at0 = w.row0 / p.group + v.lk - v.lq, w.at1 = (w.row0 + 32 * QT - 1) / p.group + v.lk - v.lq;
+    return true;
+}
 
+// The 32 rows from row0 written out.
+template <class T, int DT>
+__device__ __forceinline__ void seq_finish(const SeqAttnArgs& p, const SeqTile& w, const SeqRow& row, int row0,
+                                           SeqAcc<T, DT>& c)
+{
+    const SeqView& v = w.v;
+    const int lane = threadIdx.x & 63;
+    c.l = swap_sum(c.l);
+    // A probability of 0 does not keep out a NaN or an infinity of an unseen key in
+    // a tile that holds seen ones: such rows are done again, key by key.
+    const bool bad = row.live && !seq_finite(c);
+    T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + row.i) * p.ot + row.head * p.oh;
+    const unsigned long long all = __ballot(bad);
+    unsigned redo = (unsigned)(all | all >> 32);
+    const bool mine = (redo >> (lane & 31)) & 1;
+    if (row.live && !mine) {
+        const float inv = join_scale(c.l);
+        const int h = lane >> 5;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * d + 8 * g + 4 * h;
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = c.o[d][4 * g + e] * inv;
+                if (p.wide_out) {
+                    if (at < p.dim) store_vec<T, 4>(o + at, f);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at + e < p.dim) o[at + e] = (T)f[e];
+                }
+            }
+    }
+    while (redo) {
+        const int x = __builtin_ctz(redo);
+        redo &= redo - 1;
+        const SeqRow r = seq_row(p, row0 + x, w.rows, w.kvh);
+        float m, l, oa, oc;
+        attn_row<T>(p, v, r.i, r.head, 0, row_limit(p, v, r.i, w.prefix), m, l, oa, oc);
+        T* ro = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + r.i) * p.ot + r.head * p.oh;
+        if (lane < p.dim) ro[lane] = (T)(oa * join_scale(l));
+        if (lane + 64 < p.dim) ro[lane + 64] = (T)(oc * join_scale(l));
+    }
+}
+
+// ---- many rows: a block of four waves, QT x 32 rows each, walks the keys in stages of
+// KT x 32, two in LDS: the next one's copy runs under the present one's products.
+template <class T, int DT, int QT, int KT, int MODE>
+__device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0, unsigned char* K1, unsigned char* V0,
+                                         unsigned char* V1, unsigned* P0, unsigned* P1)
+{
+    constexpr int BK = 32 * KT;
+    SeqTile w;
+    if (!seq_tile<QT>(p, w)) return;
+    const SeqView& v = w.v;
+    const int tid = threadIdx.x, lane = tid & 63;
     u32x4 q[QT][SeqShape<T, DT>::KS];
     SeqAcc<T, DT> acc[QT];
     SeqBias bias[QT];
@@ -655,28 +760,20 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
     int limit[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        row[t] = seq_row(p, row0 + 32 * t + (lane & 31), rows, kvh);
+        row[t] = seq_row(p, w.row0 + 32 * t + (lane & 31), w.rows, w.kvh);
         load_q<T, DT>(p, v, row[t], q[t]);
-        limit[t] = row[t].live ? row_limit(p, v, row[t].i, prefix) : 0x7fffffff;
+        limit[t] = row[t].live ? row_limit(p, v, row[t].i, w.prefix) : 0x7fffffff;
         if constexpr (MODE == SEQ_BIAS || MODE == SEQ_BOTH) bias[t] = seq_bias(p, v, row[t], MODE == SEQ_BIAS);
         acc[t].init();
-    }
-    // limits rise with the row: the wave's least and largest
-    int least = 0x7fffffff, most = 0;
-    if (row0 < rows) {
-        least = row_limit(p, v, row0 / p.group, prefix);
-        const int last = row0 + 32 * QT - 1 < rows ? row0 + 32 * QT - 1 : rows - 1;
-        most = row_limit(p, v, last / p.group, prefix);
     }
 
     Stage<T, DT, BK, 256, false> sk;
     Stage<T, DT, BK, 256, true> sv;
-    sk.init((const T*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + kvh * p.kh, p.kt, v.lk, p.dim, tid);
-    sv.init((const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + kvh * p.vh, p.vt, v.lk, p.dim, tid);
+    sk.init((const T*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + w.kvh * p.kh, p.kt, v.lk, p.dim, tid);
+    sv.init((const T*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + w.kvh * p.vh, p.vt, v.lk, p.dim, tid);
     const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
-    const int at0 = row0 / p.group + v.lk - v.lq, at1 = (row0 + 32 * QT - 1) / p.group + v.lk - v.lq;
     const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
-        if (k0 >= most) return;
+        if (k0 >= w.most) return;
         f32x16 s[QT][KT];
         float rc[QT][KT];
         u32x4 pb[QT][KT][2];
@@ -684,9 +781,9 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
         for (int t = 0; t < QT; ++t)
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
-                rc[t][kt] = seq_start<MODE>(p, bias[t], s[t][kt], k0 + 32 * kt, P + 32 * kt, BK, at0, at1);
+                rc[t][kt] = seq_start<MODE>(p, bias[t], s[t][kt], k0 + 32 * kt, P + 32 * kt, BK, w.at0, w.at1);
         seq_qk<T, DT, QT, KT>(K, q, s);
-        seq_max<T, DT, QT, KT, MODE>(p, P, BK, s, rc, acc, bias, limit, k0, k0 + BK > least);
+        seq_max<T, DT, QT, KT, MODE>(p, P, BK, s, rc, acc, bias, limit, k0, k0 + BK > w.least);
         seq_exp<T, DT, QT, KT, MODE>(p, s, rc, acc, pb);
         seq_pv<T, DT, QT, KT>(V, s, pb, acc);
     };
@@ -703,16 +800,16 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
     const auto put_pos = [&](unsigned* P) {
         if (has_pos) P[tid] = pos;
     };
-    if (end > 0) {
+    if (w.end > 0) {
         issue(K0, V0, 0);
         put_pos(P0);
         __syncthreads();
-        for (int k0 = 0; k0 < end; k0 += 2 * BK) {
+        for (int k0 = 0; k0 < w.end; k0 += 2 * BK) {
             issue(K1, V1, k0 + BK);  // past the last key: zeros
             stage(K0, V0, P0, k0);
             put_pos(P1);
             __syncthreads();
-            if (k0 + BK >= end) break;
+            if (k0 + BK >= w.end) break;
             issue(K0, V0, k0 + 2 * BK);
             stage(K1, V1, P1, k0 + BK);
             put_pos(P0);
@@ -720,47 +817,181 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
         }
     }
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        SeqAcc<T, DT>& c = acc[t];
-        c.l = swap_sum(c.l);
-        // A probability of 0 does not keep out a NaN or an infinity of an unseen key in
-        // a tile that holds seen ones: such rows are done again, key by key.
-        const bool bad = row[t].live && !seq_finite(c);
-        T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + row[t].i) * p.ot + row[t].head * p.oh;
-        const unsigned long long all = __ballot(bad);
-        unsigned redo = (unsigned)(all | all >> 32);
-        const bool mine = (redo >> (lane & 31)) & 1;
-        if (row[t].live && !mine) {
-            const float inv = join_scale(c.l);
-            const int h = lane >> 5;
+    for (int t = 0; t < QT; ++t) seq_finish<T, DT>(p, w, row[t], w.row0 + 32 * t, acc[t]);
+}
+
+// ---- fp32 with many rows: the same walk on the BF16 matrix path at fp32 accuracy. Every
+// operand enters as three bf16 parts and a product as the six terms of order <= 2 (common.h),
+// 192 cycles of MFMA for 32 x 32 x 16 where FP32 MFMA takes 512. bf16 keeps fp32's range,
+// so no operand needs a scale (two f16 parts would need one: k and v have no bound here).
+// K and V go through registers, where a block splits them once for its four waves.
+template <int DT, int KT>
+struct Seq32Shape {
+    using S = SeqShape<bf16, DT>;
+    static constexpr int BK = 32 * KT;
+    static constexpr int PLANE = BK * S::ROW;          // bytes of one part of K or V
+    static constexpr int CHUNKS = BK * S::CH;          // eight elements each
+    static constexpr int N = (CHUNKS + 255) / 256;     // a thread's
+};
+
+// A thread's chunks of a stage's K or V rows, in fp32.
+template <int DT, int KT, bool V>
+struct Stage32 {
+    using X = Seq32Shape<DT, KT>;
+    using S = SeqShape<bf16, DT>;
+    const float* base;
+    long long stride;
+    int n, dim;
+    unsigned off[X::N][2];
+    f32x4 u[X::N][2];
+    __device__ __forceinline__ int row_of(int c) const { return c / S::CH; }
+    __device__ __forceinline__ int dim_of(int c) const
+    {
+        return ((c % S::CH) ^ (V ? S::vswz(row_of(c)) : S::kswz(row_of(c)))) * 8;
+    }
+    __device__ __forceinline__ void init(const float* b, long long st, int rows, int d, int tid)
+    {
+        base = b, stride = st, n = rows, dim = d;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+        for (int j = 0; j < X::N; ++j)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int at = 32 * d + 8 * g + 4 * h;
-                    float f[4];
+            for (int x = 0; x < 2; ++x) {
+                const int c = j * 256 + tid, at = dim_of(c) + 4 * x;
+                off[j][x] = c < X::CHUNKS && at < dim ? (unsigned)(row_of(c) * (int)stride + at) * 4 : 0x80000000u;
+            }
+    }
+    __device__ __forceinline__ void load(int first, int tid, int wide)
+    {
+        const int left = n - first;
+        const float* b = base + (long long)first * stride;
+        if (wide) {
+            const int rows = left < X::BK ? left : X::BK;
+            const auto rsrc = buffer_of(b, rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = c.o[d][4 * g + e] * inv;
-                    if (p.wide_out) {
-                        if (at < p.dim) store_vec<T, 4>(o + at, f);
-                    } else {
+            for (int j = 0; j < X::N; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (at + e < p.dim) o[at + e] = (T)f[e];
+                for (int x = 0; x < 2; ++x)
+                    u[j][x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[j][x], 0, 0));
+        } else {
+#pragma unroll
+            for (int j = 0; j < X::N; ++j)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = j * 256 + tid, r = row_of(c), d = dim_of(c) + 4 * x + e;
+                        u[j][x][e] = c < X::CHUNKS && r < left && d < dim ? b[(long long)r * stride + d] : 0.0f;
+                    }
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char* planes, int tid) const
+    {
+#pragma unroll
+        for (int j = 0; j < X::N; ++j) {
+            const int c = j * 256 + tid;
+            if (X::CHUNKS % 256 && c >= X::CHUNKS) break;
+            const float v[8] = {u[j][0][0], u[j][0][1], u[j][0][2], u[j][0][3], u[j][1][0], u[j][1][1], u[j][1][2], u[j][1][3]};
+            u32x4 w[3];
+            split3_x8(v, w);
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) *(u32x4*)(planes + pl * X::PLANE + c * 16) = w[pl];
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma6(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x16 c)
+{
+    c = mma16(a[2], b[0], c, bf16());
+    c = mma16(a[1], b[1], c, bf16());
+    c = mma16(a[0], b[2], c, bf16());
+    c = mma16(a[1], b[0], c, bf16());
+    c = mma16(a[0], b[1], c, bf16());
+    return mma16(a[0], b[0], c, bf16());
+}
+
+template <int DT, int KT, int MODE>
+__device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* Kp, unsigned char* Vp, unsigned* P)
+{
+    using X = Seq32Shape<DT, KT>;
+    using S = SeqShape<bf16, DT>;
+    SeqTile w;
+    if (!seq_tile<1>(p, w)) return;
+    const SeqView& v = w.v;
+    const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
+    const SeqRow row = seq_row(p, w.row0 + ql, w.rows, w.kvh);
+    u32x4 q[S::KS][3];
+    load_q32<DT>(p, v, row, q);
+    SeqAcc<float, DT> acc[1];
+    acc[0].init();
+    SeqBias bias[1];
+    if constexpr (MODE != SEQ_PLAIN) bias[0] = seq_bias(p, v, row, MODE == SEQ_BIAS);
+    const int limit[1] = {row.live ? row_limit(p, v, row.i, w.prefix) : 0x7fffffff};
+    Stage32<DT, KT, false> sk;
+    Stage32<DT, KT, true> sv;
+    sk.init((const float*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + w.kvh * p.kh, p.kt, v.lk, p.dim, tid);
+    sv.init((const float*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + w.kvh * p.vh, p.vt, v.lk, p.dim, tid);
+    const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
+    const bool has_pos = MODE != SEQ_PLAIN && p.pos_q && tid < p.axes * X::BK;
+    unsigned pos = 0;
+    const auto load = [&](int k0) {
+        if (has_pos && k0 + tid % X::BK < v.lk)
+            pos = (unsigned)pos_k[(long long)(k0 + tid % X::BK) * p.pkt + tid / X::BK * p.pka] ^ 0x80000000u;
+        sk.load(k0, tid, p.wide);
+        sv.load(k0, tid, p.wide);
+    };
+    if (w.end > 0) load(0);
+    for (int k0 = 0; k0 < w.end; k0 += X::BK) {
+        sk.put(Kp, tid);
+        sv.put(Vp, tid);
+        if (has_pos) P[tid] = pos;
+        __syncthreads();
+        load(k0 + X::BK);  // past the last key: zeros
+        if (k0 < w.most) {
+            f32x16 s[1][KT];
+            float rc[1][KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+                rc[0][kt] = seq_start<MODE>(p, bias[0], s[0][kt], k0 + 32 * kt, P + 32 * kt, X::BK, w.at0, w.at1);
+#pragma unroll
+            for (int ks = 0; ks < S::KS; ++ks) {
+                const int at = ql * S::ROW + (((2 * ks + h) ^ S::kswz(ql)) << 4);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    u32x4 a[3];
+#pragma unroll
+                    for (int pl = 0; pl < 3; ++pl) a[pl] = *(const u32x4*)(Kp + pl * X::PLANE + at + kt * 32 * S::ROW);
+                    s[0][kt] = mfma6(a, q[ks], s[0][kt]);
+                }
+            }
+            seq_max<float, DT, 1, KT, MODE>(p, P, X::BK, s, rc, acc, bias, limit, k0, k0 + X::BK > w.least);
+            u32x4 none[1][KT][2];
+            seq_exp<float, DT, 1, KT, MODE>(p, s, rc, acc, none);
+            const int x = lane & 15, kr = 4 * h + (x >> 2);
+            const int vrow = kr * S::ROW + (x & 1) * 8;
+            const int lc = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1), vsw = S::vswz(kr);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = s[0][kt][8 * st + j];
+                    u32x4 b[3];
+                    split3_x8(f, b);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        u32x4 a[3];
+#pragma unroll
+                        for (int pl = 0; pl < 3; ++pl)
+                            a[pl] = read_v(Vp + pl * X::PLANE + vrow + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW,
+                                           8 * S::ROW);
+                        acc[0].o[d] = mfma6(a, b, acc[0].o[d]);
                     }
                 }
         }
-        while (redo) {
-            const int x = __builtin_ctz(redo);
-            redo &= redo - 1;
-            const SeqRow r = seq_row(p, row0 + 32 * t + x, rows, kvh);
-            float m, l, oa, oc;
-            attn_row<T>(p, v, r.i, r.head, 0, row_limit(p, v, r.i, prefix), m, l, oa, oc);
-            T* ro = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + r.i) * p.ot + r.head * p.oh;
-            if (lane < p.dim) ro[lane] = (T)(oa * join_scale(l));
-            if (lane + 64 < p.dim) ro[lane + 64] = (T)(oc * join_scale(l));
-        }
+        __syncthreads();  // the stage has been read
     }
+    seq_finish<float, DT>(p, w, row, w.row0, acc[0]);
 }
 
 // ---- few rows a sequence (a token each, say) against many keys: the keys go over blocks
@@ -1047,18 +1278,27 @@ SEQ_INST(hat_attnseq_bf16_d1_both, bf16, 1, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d2_both, bf16, 2, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d3_both, bf16, 3, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f32_d1, float, 1, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_f32_d1_bias, float, 1, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f32_d1_both, float, 1, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f32_d2, float, 2, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_f32_d2_bias, float, 2, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f32_d2_both, float, 2, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f32_d3, float, 3, 1, 1, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_f32_d3_bias, float, 3, 1, 1, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f32_d3_both, float, 3, 1, 1, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f32_d4, float, 4, 1, 1, SEQ_PLAIN, 1)
-SEQ_INST(hat_attnseq_f32_d4_bias, float, 4, 1, 1, SEQ_BIAS, 1)
-SEQ_INST(hat_attnseq_f32_d4_both, float, 4, 1, 1, SEQ_BOTH, 1)
+#define SEQ32_INST(NAME, DT, KT, MODE, WPS)                                                                   \
+    extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
+    {                                                                                                        \
+        constexpr int B = 3 * Seq32Shape<DT, KT>::PLANE;                                                     \
+        __shared__ __attribute__((aligned(16))) unsigned char K[B], V[B];                                    \
+        __shared__ __attribute__((aligned(16))) unsigned P[MODE == SEQ_PLAIN ? 4 : 128 * KT];                \
+        seq32_body<DT, KT, MODE>(p, K, V, P);                                                                \
+    }
+
+SEQ32_INST(hat_attnseq_f32_d1, 1, 2, SEQ_PLAIN, 2)
+SEQ32_INST(hat_attnseq_f32_d1_bias, 1, 2, SEQ_BIAS, 2)
+SEQ32_INST(hat_attnseq_f32_d1_both, 1, 2, SEQ_BOTH, 2)
+SEQ32_INST(hat_attnseq_f32_d2, 2, 2, SEQ_PLAIN, 2)
+SEQ32_INST(hat_attnseq_f32_d2_bias, 2, 2, SEQ_BIAS, 2)
+SEQ32_INST(hat_attnseq_f32_d2_both, 2, 2, SEQ_BOTH, 2)
+SEQ32_INST(hat_attnseq_f32_d3, 3, 1, SEQ_PLAIN, 2)
+SEQ32_INST(hat_attnseq_f32_d3_bias, 3, 1, SEQ_BIAS, 2)
+SEQ32_INST(hat_attnseq_f32_d3_both, 3, 1, SEQ_BOTH, 2)
+SEQ32_INST(hat_attnseq_f32_d4, 4, 1, SEQ_PLAIN, 2)
+SEQ32_INST(hat_attnseq_f32_d4_bias, 4, 1, SEQ_BIAS, 2)
+SEQ32_INST(hat_attnseq_f32_d4_both, 4, 1, SEQ_BOTH, 2)
 
 #define SPLIT_INST(NAME, T, DT, W)                                                                           \
     extern "C" __global__ __launch_bounds__(64 * W, 1) void NAME(SeqAttnArgs p)                              \

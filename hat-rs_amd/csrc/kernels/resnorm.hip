@@ -58,6 +58,14 @@ struct Row {
             if ((i * TPR + t) * V < width) load_vec<T, V>(p + (i * TPR + t) * V, v);
         }
     }
+    __device__ __forceinline__ typename Vec<T, V>::type raw(int i) const
+    {
+        if constexpr (TPR >= 64)
+            return buffer_load_raw<T, V>(r, t * V * (int)sizeof(T), i * TPR * V * (int)sizeof(T));
+        else
+            return (i * TPR + t) * V < width ? *(const typename Vec<T, V>::type*)(p + (i * TPR + t) * V)
+                                             : (typename Vec<T, V>::type)(T)0.0f;
+    }
     __device__ __forceinline__ void store(int i, const float (&v)[V]) const
     {
         if constexpr (TPR >= 64) {
@@ -117,6 +125,11 @@ __device__ __forceinline__ void resnorm_body(const ResNormArgs& p)
     const long long row = (long long)blockIdx.x * (THREADS / TPR) + in_block;
     if (row >= p.rows) return;  // whole rows leave; with more than a wave a row, whole blocks
     float v[NV][V];
+    const Row<T, TPR, V> x(p.x, row * p.xs, p.width, t), xo(p.xo, row * p.xos, p.width, t);
+    // x is read before y's sums, as it came: its loads run under them
+    typename Vec<T, V>::type xr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xr[i] = x.raw(i);
     if (p.y) {
         const Row<T, TPR, V> y(p.y, row * p.ys, p.width, t);
 #pragma unroll
@@ -133,11 +146,10 @@ __device__ __forceinline__ void resnorm_body(const ResNormArgs& p)
             }
         }
     }
-    const Row<T, TPR, V> x(p.x, row * p.xs, p.width, t), xo(p.xo, row * p.xos, p.width, t);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float u[V];
-        x.load(i, u);
+        to_float<T, V>(xr[i], u);
         if (p.y) {
 #pragma unroll
             for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(p.scale, v[i][j], u[j]);

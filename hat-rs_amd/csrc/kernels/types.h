@@ -44,23 +44,34 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[N])
 // N consecutive elements at byte offset off + base of a buffer descriptor: zeros past its
 // end, where stores are dropped, so that a row's last moves need no branch.
 template <class T, int N>
-__device__ __forceinline__ void buffer_load_vec(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base, float (&v)[N])
+__device__ __forceinline__ typename Vec<T, N>::type buffer_load_raw(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base)
 {
-    typename Vec<T, N>::type u;
+    typedef typename Vec<T, N>::type U;
     if constexpr (sizeof(T) * N == 16)
-        u = __builtin_bit_cast(decltype(u), __builtin_amdgcn_raw_buffer_load_b128(r, off, base, 0));
+        return __builtin_bit_cast(U, __builtin_amdgcn_raw_buffer_load_b128(r, off, base, 0));
     else if constexpr (sizeof(T) * N == 8)
-        u = __builtin_bit_cast(decltype(u), __builtin_amdgcn_raw_buffer_load_b64(r, off, base, 0));
+        return __builtin_bit_cast(U, __builtin_amdgcn_raw_buffer_load_b64(r, off, base, 0));
     else if constexpr (sizeof(T) * N == 4)
-        u = __builtin_bit_cast(decltype(u), __builtin_amdgcn_raw_buffer_load_b32(r, off, base, 0));
+        return __builtin_bit_cast(U, __builtin_amdgcn_raw_buffer_load_b32(r, off, base, 0));
     else
-        u = __builtin_bit_cast(decltype(u), __builtin_amdgcn_raw_buffer_load_b16(r, off, base, 0));
+        return __builtin_bit_cast(U, __builtin_amdgcn_raw_buffer_load_b16(r, off, base, 0));
+}
+
+template <class T, int N>
+__device__ __forceinline__ void to_float(const typename Vec<T, N>::type& u, float (&v)[N])
+{
     if constexpr (N == 1) {
         v[0] = (float)u;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = (float)u[i];
     }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void buffer_load_vec(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned base, float (&v)[N])
+{
+    to_float<T, N>(buffer_load_raw<T, N>(r, off, base), v);
 }
 
 template <class T, int N>
