@@ -53,11 +53,13 @@ const std::vector<std::string>& required_kernels()
         "hat_attnseq_f32_d1_split", "hat_attnseq_f32_d2_split", "hat_attnseq_f32_d3_split", "hat_attnseq_f32_d4_split",
         "hat_attnseq_join_f32", "hat_attnseq_join_f16", "hat_attnseq_join_bf16",
         "hat_resnorm_f32_16", "hat_resnorm_f32_64", "hat_resnorm_f32_256", "hat_resnorm_f32_1024",
-        "hat_resnorm_f32_64e", "hat_resnorm_f32_1024e",
+        "hat_resnorm_f32_64e", "hat_resnorm_f32_256e", "hat_resnorm_f32_1024e",
         "hat_resnorm_f16_16", "hat_resnorm_f16_64", "hat_resnorm_f16_256", "hat_resnorm_f16_1024",
-        "hat_resnorm_f16_64h", "hat_resnorm_f16_1024h", "hat_resnorm_f16_64e", "hat_resnorm_f16_1024e",
+        "hat_resnorm_f16_64h", "hat_resnorm_f16_256h", "hat_resnorm_f16_1024h", "hat_resnorm_f16_64e",
+        "hat_resnorm_f16_256e", "hat_resnorm_f16_1024e",
         "hat_resnorm_bf16_16", "hat_resnorm_bf16_64", "hat_resnorm_bf16_256", "hat_resnorm_bf16_1024",
-        "hat_resnorm_bf16_64h", "hat_resnorm_bf16_1024h", "hat_resnorm_bf16_64e", "hat_resnorm_bf16_1024e",
+        "hat_resnorm_bf16_64h", "hat_resnorm_bf16_256h", "hat_resnorm_bf16_1024h", "hat_resnorm_bf16_64e",
+        "hat_resnorm_bf16_256e", "hat_resnorm_bf16_1024e",
     };
     return k;
 }

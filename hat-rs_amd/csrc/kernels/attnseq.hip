@@ -1278,7 +1278,7 @@ SEQ_INST(hat_attnseq_bf16_d1_both, bf16, 1, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d2_both, bf16, 2, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d3_both, bf16, 3, 1, 2, SEQ_BOTH, 2)
 SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 1, 2, SEQ_BOTH, 2)
-#define SEQ32_INST(NAME, DT, KT, MODE, WPS)                                                                   \
+#define SEQ_FP_INST(NAME, DT, KT, MODE, WPS)                                                                   \
     extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
     {                                                                                                        \
         constexpr int B = 3 * Seq32Shape<DT, KT>::PLANE;                                                     \
@@ -1287,18 +1287,18 @@ SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 1, 2, SEQ_BOTH, 2)
         seq32_body<DT, KT, MODE>(p, K, V, P);                                                                \
     }
 
-SEQ32_INST(hat_attnseq_f32_d1, 1, 2, SEQ_PLAIN, 2)
-SEQ32_INST(hat_attnseq_f32_d1_bias, 1, 2, SEQ_BIAS, 2)
-SEQ32_INST(hat_attnseq_f32_d1_both, 1, 2, SEQ_BOTH, 2)
-SEQ32_INST(hat_attnseq_f32_d2, 2, 2, SEQ_PLAIN, 2)
-SEQ32_INST(hat_attnseq_f32_d2_bias, 2, 2, SEQ_BIAS, 2)
-SEQ32_INST(hat_attnseq_f32_d2_both, 2, 2, SEQ_BOTH, 2)
-SEQ32_INST(hat_attnseq_f32_d3, 3, 1, SEQ_PLAIN, 2)
-SEQ32_INST(hat_attnseq_f32_d3_bias, 3, 1, SEQ_BIAS, 2)
-SEQ32_INST(hat_attnseq_f32_d3_both, 3, 1, SEQ_BOTH, 2)
-SEQ32_INST(hat_attnseq_f32_d4, 4, 1, SEQ_PLAIN, 2)
-SEQ32_INST(hat_attnseq_f32_d4_bias, 4, 1, SEQ_BIAS, 2)
-SEQ32_INST(hat_attnseq_f32_d4_both, 4, 1, SEQ_BOTH, 2)
+SEQ_FP_INST(hat_attnseq_f32_d1, 1, 2, SEQ_PLAIN, 2)
+SEQ_FP_INST(hat_attnseq_f32_d1_bias, 1, 2, SEQ_BIAS, 2)
+SEQ_FP_INST(hat_attnseq_f32_d1_both, 1, 2, SEQ_BOTH, 2)
+SEQ_FP_INST(hat_attnseq_f32_d2, 2, 2, SEQ_PLAIN, 2)
+SEQ_FP_INST(hat_attnseq_f32_d2_bias, 2, 2, SEQ_BIAS, 2)
+SEQ_FP_INST(hat_attnseq_f32_d2_both, 2, 2, SEQ_BOTH, 2)
+SEQ_FP_INST(hat_attnseq_f32_d3, 3, 1, SEQ_PLAIN, 2)
+SEQ_FP_INST(hat_attnseq_f32_d3_bias, 3, 1, SEQ_BIAS, 2)
+SEQ_FP_INST(hat_attnseq_f32_d3_both, 3, 1, SEQ_BOTH, 2)
+SEQ_FP_INST(hat_attnseq_f32_d4, 4, 1, SEQ_PLAIN, 2)
+SEQ_FP_INST(hat_attnseq_f32_d4_bias, 4, 1, SEQ_BIAS, 2)
+SEQ_FP_INST(hat_attnseq_f32_d4_both, 4, 1, SEQ_BOTH, 2)
 
 #define SPLIT_INST(NAME, T, DT, W)                                                                           \
     extern "C" __global__ __launch_bounds__(64 * W, 1) void NAME(SeqAttnArgs p)                              \
@@ -1311,15 +1311,15 @@ SEQ32_INST(hat_attnseq_f32_d4_both, 4, 1, SEQ_BOTH, 2)
         seq_split_body<T, DT, W>(p, B0, B1, B2, B3, P0, P1, ml, &flags);                                     \
     }
 
-SPLIT_INST(hat_attnseq_f16_d1_split, f16, 1, 4)
-SPLIT_INST(hat_attnseq_f16_d2_split, f16, 2, 4)
+SPLIT_INST(hat_attnseq_f16_d1_split, f16, 1, 8)
+SPLIT_INST(hat_attnseq_f16_d2_split, f16, 2, 8)
 SPLIT_INST(hat_attnseq_f16_d3_split, f16, 3, 4)
 SPLIT_INST(hat_attnseq_f16_d4_split, f16, 4, 4)
-SPLIT_INST(hat_attnseq_bf16_d1_split, bf16, 1, 4)
-SPLIT_INST(hat_attnseq_bf16_d2_split, bf16, 2, 4)
+SPLIT_INST(hat_attnseq_bf16_d1_split, bf16, 1, 8)
+SPLIT_INST(hat_attnseq_bf16_d2_split, bf16, 2, 8)
 SPLIT_INST(hat_attnseq_bf16_d3_split, bf16, 3, 4)
 SPLIT_INST(hat_attnseq_bf16_d4_split, bf16, 4, 4)
-SPLIT_INST(hat_attnseq_f32_d1_split, float, 1, 4)
+SPLIT_INST(hat_attnseq_f32_d1_split, float, 1, 8)
 SPLIT_INST(hat_attnseq_f32_d2_split, float, 2, 4)
 SPLIT_INST(hat_attnseq_f32_d3_split, float, 3, 2)
 SPLIT_INST(hat_attnseq_f32_d4_split, float, 4, 2)

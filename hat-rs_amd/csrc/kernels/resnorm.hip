@@ -81,19 +81,22 @@ template <int TPR, int V, int NV>
 __device__ __forceinline__ void row_norm(float (&v)[NV][V], int kind, const float* w, const float* b, float eps,
                                          int width, int t, float* lds)
 {
+    // The mean is 0 for RMSNorm and taken off all the same: with the subtraction under the
+    // condition the compiler lost the values on the other path (f16, one vector a thread).
+    float mean = 0.0f;
     if (kind == NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[i][j];
-        const float mean = row_sum<TPR>(s, lds) / (float)width;
+        mean = row_sum<TPR>(s, lds) / (float)width;
+    }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const float m = (i * TPR + t) * V < width ? mean : 0.0f;
+    for (int i = 0; i < NV; ++i) {
+        const float m = (i * TPR + t) * V < width ? mean : 0.0f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] -= m;
-        }
+        for (int j = 0; j < V; ++j) v[i][j] -= m;
     }
     float q = 0.0f;
 #pragma unroll
@@ -165,8 +168,34 @@ __device__ __forceinline__ void resnorm_body(const ResNormArgs& p)
     for (int i = 0; i < NV; ++i) h.store(i, v[i]);
 }
 
+// NV: the most vectors a thread. The body is compiled for fewer as well, since moves past
+// the row's end cost their issue (57600 rows of 1024 in bf16: 178 us with two of four in
+// use, ... with two).
+template <class T, int THREADS, int TPR, int V, int NV>
+__device__ __forceinline__ void resnorm_kernel(const ResNormArgs& p)
+{
+    const int n = (p.width + TPR * V - 1) / (TPR * V);
+    if constexpr (NV >= 8) {
+        if (n <= NV / 4)
+            resnorm_body<T, THREADS, TPR, V, NV / 4>(p);
+        else if (n <= NV / 2)
+            resnorm_body<T, THREADS, TPR, V, NV / 2>(p);
+        else
+            resnorm_body<T, THREADS, TPR, V, NV>(p);
+    } else {
+        if (n == 1)
+            resnorm_body<T, THREADS, TPR, V, 1>(p);
+        else if (n == 2)
+            resnorm_body<T, THREADS, TPR, V, 2>(p);
+        else if (NV == 4 && n == 3)
+            resnorm_body<T, THREADS, TPR, V, 3>(p);
+        else
+            resnorm_body<T, THREADS, TPR, V, NV>(p);
+    }
+}
+
 #define RESNORM_INST(NAME, T, THREADS, TPR, V, NV) \
-    extern "C" __global__ __launch_bounds__(THREADS) void NAME(ResNormArgs p) { resnorm_body<T, THREADS, TPR, V, NV>(p); }
+    extern "C" __global__ __launch_bounds__(THREADS) void NAME(ResNormArgs p) { resnorm_kernel<T, THREADS, TPR, V, NV>(p); }
 
 // by the bytes of a move (16; 4 or one element where the rows' alignment or width allow
 // no more) and the threads a row
@@ -175,20 +204,25 @@ RESNORM_INST(hat_resnorm_f32_64, float, 256, 64, 4, 4)
 RESNORM_INST(hat_resnorm_f32_256, float, 256, 256, 4, 4)
 RESNORM_INST(hat_resnorm_f32_1024, float, 1024, 1024, 4, 4)
 RESNORM_INST(hat_resnorm_f32_64e, float, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_f32_256e, float, 256, 256, 1, 16)
 RESNORM_INST(hat_resnorm_f32_1024e, float, 1024, 1024, 1, 16)
 RESNORM_INST(hat_resnorm_f16_16, f16, 256, 16, 8, 2)
 RESNORM_INST(hat_resnorm_f16_64, f16, 256, 64, 8, 4)
 RESNORM_INST(hat_resnorm_f16_256, f16, 256, 256, 8, 4)
 RESNORM_INST(hat_resnorm_f16_1024, f16, 1024, 1024, 8, 2)
 RESNORM_INST(hat_resnorm_f16_64h, f16, 256, 64, 2, 8)
+RESNORM_INST(hat_resnorm_f16_256h, f16, 256, 256, 2, 8)
 RESNORM_INST(hat_resnorm_f16_1024h, f16, 1024, 1024, 2, 8)
 RESNORM_INST(hat_resnorm_f16_64e, f16, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_f16_256e, f16, 256, 256, 1, 16)
 RESNORM_INST(hat_resnorm_f16_1024e, f16, 1024, 1024, 1, 16)
 RESNORM_INST(hat_resnorm_bf16_16, bf16, 256, 16, 8, 2)
 RESNORM_INST(hat_resnorm_bf16_64, bf16, 256, 64, 8, 4)
 RESNORM_INST(hat_resnorm_bf16_256, bf16, 256, 256, 8, 4)
 RESNORM_INST(hat_resnorm_bf16_1024, bf16, 1024, 1024, 8, 2)
 RESNORM_INST(hat_resnorm_bf16_64h, bf16, 256, 64, 2, 8)
+RESNORM_INST(hat_resnorm_bf16_256h, bf16, 256, 256, 2, 8)
 RESNORM_INST(hat_resnorm_bf16_1024h, bf16, 1024, 1024, 2, 8)
 RESNORM_INST(hat_resnorm_bf16_64e, bf16, 256, 64, 1, 16)
+RESNORM_INST(hat_resnorm_bf16_256e, bf16, 256, 256, 1, 16)
 RESNORM_INST(hat_resnorm_bf16_1024e, bf16, 1024, 1024, 1, 16)

@@ -17,7 +17,6 @@ using namespace hatk;
 #define ROT_THREADS 256
 #define ROT_ANGLES 4096  // cos and sin values a block keeps (32 KB)
 #define ROT_TOKENS 64    // tokens a block takes at most
-#define ROT_AHEAD 4
 
 // n / d for n < 2^20 by d's reciprocal: the error of (n + 1/2) / d is below 2^-2 / d.
 __device__ __forceinline__ int div_small(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
@@ -25,7 +24,7 @@ __device__ __forceinline__ int div_small(int n, float inv) { return (int)(((floa
 template <class T, int V>
 __device__ __forceinline__ void rotary_body(const RotaryArgs& p)
 {
-    __shared__ __attribute__((aligned(16))) float cs[ROT_ANGLES], sn[ROT_ANGLES];
+    __shared__ __attribute__((aligned(16))) f32x2 cs[ROT_ANGLES];  // (cos, sin)
     const long long first = (long long)blockIdx.x * p.per;
     const long long all = p.tokens * p.batch;
     const int n = (int)(all - first < p.per ? all - first : p.per);
@@ -38,8 +37,7 @@ __device__ __forceinline__ void rotary_body(const RotaryArgs& p)
         const double turns = (double)p.pos[b * p.pb + tok * p.pt + axis * p.pa] * p.turn[i];
         float s, c;
         sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &s, &c);
-        cs[e] = c;
-        sn[e] = s;
+        cs[e] = (f32x2){c, s};
     }
     // where the block's tokens lie in x and y
     __shared__ long long at[4][ROT_TOKENS];
@@ -52,70 +50,82 @@ __device__ __forceinline__ void rotary_body(const RotaryArgs& p)
         }
     }
     __syncthreads();
-    const int turned = p.neighbours && V > 1 ? 2 * p.pairs / V : p.pairs / V;
+    // An item is two moves of V elements: the halves of V pairs, two neighbouring runs, or
+    // two runs of the dims behind the rotated ones. All take the same path, as a branch
+    // would cost a wave both: the runs without an angle keep their bits at the end.
+    const int turned = p.neighbours ? (2 * p.pairs / V + 1) / 2 : p.pairs / V;
+    const int rest = p.dim / V - 2 * p.pairs / V;  // moves behind the rotated dims
     const int per_token = p.chunks * (p.heads[0] + p.heads[1]);
     const int all_items = n * per_token;
     typedef typename Vec<T, V>::type vec;
-    // ROT_AHEAD items a thread at a time, their loads issued before the first is used
+    // items a thread loads before it stores the first: 57600 tokens, 24 heads of 64 in 16-byte
+    // moves 77 us by one, 72 by two, 75 by four; of 72 in 8-byte moves 112, 95, 89 (six: 92)
+    constexpr int ROT_AHEAD = sizeof(T) * V >= 16 ? 2 : 4;
     for (int e0 = threadIdx.x; e0 < all_items; e0 += ROT_THREADS * ROT_AHEAD) {
         vec u[ROT_AHEAD], v[ROT_AHEAD];
         T* y[ROT_AHEAD];
-        int c[ROT_AHEAD], angle[ROT_AHEAD];  // c < 0: no item
+        int d0[ROT_AHEAD], d1[ROT_AHEAD], angle[ROT_AHEAD];  // angle < 0: a copy; d0 < 0: no item
 #pragma unroll
         for (int k = 0; k < ROT_AHEAD; ++k) {
             const int e = e0 + k * ROT_THREADS;
-            c[k] = -1;
+            d0[k] = -1;
             if (e >= all_items) continue;
             const int t = div_small(e, p.inv_items), r = e - t * per_token;
             int head = div_small(r, p.inv_chunks);
-            c[k] = r - head * p.chunks;
-            angle[k] = t * p.pairs;
+            const int c = r - head * p.chunks;
             const int w = head >= p.heads[0];
             head -= w ? p.heads[0] : 0;
             const T* x = (const T*)p.x[w] + at[w][t] + head * p.xh[w];
             y[k] = (T*)p.y[w] + at[2 + w][t] + head * p.yh[w];
-            if (V == 1 && p.neighbours && c[k] < turned) {
-                u[k] = *(const vec*)(x + 2 * c[k]);
-                v[k] = *(const vec*)(x + 2 * c[k] + 1);
+            if (c >= turned) {
+                const int i = c - turned, j = i + (rest + 1) / 2;
+                d0[k] = 2 * p.pairs + i * V;
+                d1[k] = 2 * p.pairs + (j < rest ? j : i) * V;  // an odd one twice
+                angle[k] = -1;
+            } else if (p.neighbours) {
+                d0[k] = 2 * c * V;
+                d1[k] = d0[k] + V < 2 * p.pairs ? d0[k] + V : d0[k];
+                angle[k] = t * p.pairs;
             } else {
-                const int d = c[k] < turned ? c[k] * V : 2 * p.pairs + (c[k] - turned) * V;
-                u[k] = *(const vec*)(x + d);
-                if (!p.neighbours && c[k] < turned) v[k] = *(const vec*)(x + d + p.pairs);
+                d0[k] = c * V;
+                d1[k] = d0[k] + p.pairs;
+                angle[k] = t * p.pairs + d0[k];
             }
+            u[k] = *(const vec*)(x + d0[k]);
+            v[k] = *(const vec*)(x + d1[k]);
         }
 #pragma unroll
         for (int k = 0; k < ROT_AHEAD; ++k) {
-            if (c[k] < 0) continue;
-            if (c[k] >= turned) {  // behind the rotated dims
-                *(vec*)(y[k] + 2 * p.pairs + (c[k] - turned) * V) = u[k];
-            } else if (!p.neighbours || V == 1) {
-                const int i = c[k] * V;
-                float uo[V], vo[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float a, b;
-                    if constexpr (V == 1)
-                        a = (float)u[k], b = (float)v[k];
-                    else
-                        a = (float)u[k][j], b = (float)v[k][j];
-                    const float cj = cs[angle[k] + i + j], sj = sn[angle[k] + i + j];
-                    uo[j] = a * cj - b * sj;
-                    vo[j] = b * cj + a * sj;
-                }
-                store_vec<T, V>(y[k] + (V == 1 && p.neighbours ? 2 * i : i), uo);
-                store_vec<T, V>(y[k] + (V == 1 && p.neighbours ? 2 * i + 1 : i + p.pairs), vo);
-            } else if constexpr (V > 1) {
-                const int d = c[k] * V;
-                float o[V];
+            if (d0[k] < 0) continue;
+            const bool copy = angle[k] < 0;
+            vec uo, vo;
+            if constexpr (V == 1) {
+                // neighbours too are a pair: turned counts pairs here
+                const f32x2 a = cs[copy ? 0 : p.neighbours ? angle[k] + d0[k] / 2 : angle[k]];
+                const float f = (float)u[k], g = (float)v[k];
+                uo = (T)(f * a[0] - g * a[1]);
+                vo = (T)(g * a[0] + f * a[1]);
+            } else if (p.neighbours) {
 #pragma unroll
                 for (int j = 0; j < V; j += 2) {
-                    const float a = (float)u[k][j], b = (float)u[k][j + 1];
-                    const float cj = cs[angle[k] + (d + j) / 2], sj = sn[angle[k] + (d + j) / 2];
-                    o[j] = a * cj - b * sj;
-                    o[j + 1] = b * cj + a * sj;
+                    const f32x2 a = cs[copy ? 0 : angle[k] + (d0[k] + j) / 2], b = cs[copy ? 0 : angle[k] + (d1[k] + j) / 2];
+                    const float f = (float)u[k][j], g = (float)u[k][j + 1], h = (float)v[k][j], i = (float)v[k][j + 1];
+                    uo[j] = (T)(f * a[0] - g * a[1]);
+                    uo[j + 1] = (T)(g * a[0] + f * a[1]);
+                    vo[j] = (T)(h * b[0] - i * b[1]);
+                    vo[j + 1] = (T)(i * b[0] + h * b[1]);
                 }
-                store_vec<T, V>(y[k] + d, o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const f32x2 a = cs[(copy ? 0 : angle[k]) + j];
+                    const float f = (float)u[k][j], g = (float)v[k][j];
+                    uo[j] = (T)(f * a[0] - g * a[1]);
+                    vo[j] = (T)(g * a[0] + f * a[1]);
+                }
             }
+            *(vec*)(y[k] + d0[k]) = copy ? u[k] : uo;
+            *(vec*)(y[k] + d1[k]) = copy ? v[k] : vo;
         }
     }
 }

@@ -166,9 +166,9 @@ void op_rotary(const hat_rotary* a, void* stream)
     p.pos = a->pos.data, p.pb = a->pos.batch_stride, p.pt = a->pos.token_stride, p.pa = a->pos.axis_stride;
     p.tokens = a->tokens, p.batch = a->batch;
     p.dim = a->head_dim, p.pairs = pairs, p.neighbours = a->neighbours != 0;
-    const int turned = a->neighbours && V > 1 ? 2 * pairs / V : pairs / V;
+    const int turned = a->neighbours ? (2 * pairs / V + 1) / 2 : pairs / V;
     const int rest = in_place ? 0 : (a->head_dim - 2 * pairs) / V;  // in place they are there already
-    p.chunks = turned + rest;
+    p.chunks = turned + (rest + 1) / 2;
     const int items = p.chunks * (heads[0] + heads[1]);
     int n = 0;
     for (int x = 0; x < a->axes; ++x)
@@ -238,6 +238,13 @@ struct AttnPlan {
 
 int dim_tiles(const hat_attention* a) { return (a->head_dim + 31) / 32; }
 
+// Waves a block of the split kernels (SPLIT_INST): as many as their LDS allows.
+int split_waves(const hat_attention* a)
+{
+    const int dt = dim_tiles(a);
+    return a->dtype == HAT_F32 ? (dt == 1 ? 8 : dt == 2 ? 4 : 2) : dt <= 2 ? 8 : 4;
+}
+
 AttnPlan attn_plan(const hat_attention* a)
 {
     AttnPlan p{};
@@ -257,10 +264,16 @@ AttnPlan attn_plan(const hat_attention* a)
         p.chunk = 1 << 30;
         return p;
     }
-    // Enough chunks that every CU has two blocks, of 256 keys at least.
+    // Chunks of keys. A block fills a CU's LDS, so 256 blocks are a round; lengths that the
+    // host does not know may leave most of a chunk empty, so they get eight rounds of
+    // smaller ones. (16 sequences of 16384 keys, 8 heads of 128: 182 us in 256 blocks, 188
+    // in 512, 200 in 1024.) Up to 128 keys a wave one chunk costs less than the join's
+    // launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
     const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
     const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
-    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / 512 + 127) / 128 * 128));
+    const long long blocks = a->cu_k || a->k_lens ? 2048 : 256, whole = 128 * split_waves(a);
+    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / blocks + 127) / 128 * 128));
+    if (a->k_tokens <= whole) p.chunk = (int)whole;
     const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
     const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
     p.slots = (int)(a->cu_k ? slots : std::max<long long>(n, 1));
@@ -353,7 +366,7 @@ void op_attention(const hat_attention* a, void* stream)
     else if (a->slopes)
         name += p.c1 > 1e-6f ? "_bias" : "_both";
     p.fold = p.causal && !a->cu_q && plan.blocks <= 1024;
-    const int threads = plan.split && a->dtype == HAT_F32 && dim_tiles(a) > 2 ? 128 : 256;
+    const int threads = plan.split ? 64 * split_waves(a) : 256;
     launch(s, name.c_str(), grid_of(op, plan.blocks), 1, 1, threads, p);
     if (plan.join_rows)
         launch(s, ("hat_attnseq_join_" + type).c_str(), grid_of(op, (plan.join_rows + 3) / 4), 1, 1, 256, p);
@@ -417,21 +430,22 @@ void op_residual_norm(const hat_residual_norm* a, void* stream)
     p.rows = a->rows, p.rows_per_gate = a->gate ? a->rows_per_gate : 1;
     p.width = a->width, p.post = a->post, p.pre = a->pre;
     p.scale = a->scale, p.post_eps = a->post_eps, p.pre_eps = a->pre_eps;
-    // The fewest threads a row whose registers hold it.
+    // The fewest threads a row whose registers hold it (resnorm.hip): no barrier up to a
+    // wave, and a 1024-thread block costs twice a 256-thread one (8192 in bf16: 257 us
+    // against 135).
     const int W = a->width;
-    const char* form;
-    int per, threads = 256;
-    if (move < 16)
-        form = move > e ? (W <= 1024 ? "64h" : "1024h") : W <= 1024 ? "64e" : "1024e", per = W <= 1024 ? 4 : 1;
-    else if (W <= (a->dtype == HAT_F32 ? 192 : 256))
+    const bool vec = move == 16;
+    std::string form;
+    int per = 1, threads = 256;
+    if (vec && W <= (e == 4 ? 192 : 256))
         form = "16", per = 16;
-    else if (W <= (a->dtype == HAT_F32 ? 1024 : 2048))
+    else if (W <= (vec ? 64 * 4 * 16 / (int)e : 1024))
         form = "64", per = 4;
-    else if (W <= (a->dtype == HAT_F32 ? 4096 : 8192))
-        form = "256", per = 1;
+    else if (W <= (vec ? 256 * 4 * 16 / (int)e : 4096))
+        form = "256";
     else
-        form = "1024", per = 1;
-    if (form[0] == '1' && form[1] == '0') threads = 1024;
+        form = "1024", threads = 1024;
+    if (!vec) form += move > e ? "h" : "e";
     const DeviceScope scope;
     hipStream_t s = check_stream(op, stream);
     const std::string name = std::string("hat_resnorm_") + type_name(a->dtype) + "_" + form;

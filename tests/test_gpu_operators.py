@@ -252,6 +252,38 @@ def test_residual_norm(hl, kind, case):
     assert torch.equal(xd, xo) and torch.equal(yd, h)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("width", [16, 130, 264, 600, 1001, 1030, 1536, 2047, 4100, 6000, 9000, 9002])
+def test_residual_norm_every_combination(hl, kind, width):
+    """Each norm before with each norm behind, with and without a gate and weights, for
+    every number of threads a row and vectors a thread."""
+    t, g, rows = TYPES[kind], _gen(width), 6
+    print(f"residual_norm {kind} {width}", flush=True)
+    x, y = _randn(g, t, rows, width, std=2.0).cuda(), _randn(g, t, rows, width).cuda()
+    gate = torch.sigmoid(_randn(g, t, 2, width).float()).to(t).cuda()
+    w, b = (_randn(g, torch.float32, width, std=0.5).cuda() + 1.0 for _ in range(2))
+    for post in ("none", "layer", "rms"):
+        for pre in ("none", "layer", "rms"):
+            for gated in (False, True):
+                for weights in ((None, None), (w, None), (w, b)):
+                    xo, h = torch.full_like(x, 3.0), torch.full_like(x, 3.0)
+                    pw, pb = weights if post != "none" else (None, None)
+                    nw, nb = weights if pre != "none" else (None, None)
+                    hl.op_residual_norm(x, y, xo, h, gate=gate if gated else None, scale=0.375, post=post,
+                                        post_weight=pw, post_bias=pb, pre=pre, pre_weight=nw, pre_bias=nb)
+                    def norm(v, kind, w, b):
+                        v = v - v.mean(1, keepdim=True) if kind == "layer" else v
+                        v = v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-5) if kind != "none" else v
+                        v = v * w.double() if w is not None else v
+                        return v + b.double() if b is not None else v
+                    add = norm(y.double(), post, pw, pb) * (gate.double().repeat_interleave(3, 0) if gated else 1.0)
+                    want = x.double() + 0.375 * add
+                    # values of up to ten units and sums in fp32 (see above): 400 u of ten
+                    for got, true in ((xo, want), (h, norm(want, pre, nw, nb))):
+                        off = (got.double() - true).abs() - U(t) * 1.01 * true.abs()
+                        assert off.max() <= 4000 * u, (post, pre, gated, weights[0] is not None, weights[1] is not None)
+
+
 def test_residual_norm_of_the_stream_alone(hl):
     """y left out: a norm of x, at the width the forward's own LayerNorm has."""
     g = _gen(3)
