@@ -401,7 +401,7 @@ struct SeqAttnArgs {
     int n_seq, q_heads, kv_heads, group, dim, axes;
     int q_tokens, k_tokens;  // of a batch entry, or of the packed tensor
     int causal, fold;
-    int wide;                // q, k, v rows: 16-byte chunks (else element by element)
+    int wide;                // q, k, v rows in moves of 16 bytes (2), 4 bytes (1) or an element (0)
     int wide_out;            // out rows: four elements at a time
     float scale;             // scores = scale * q . k
     float cap, inv_cap;      // cap > 0: cap * tanh(scores * inv_cap)

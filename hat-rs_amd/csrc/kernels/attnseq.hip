@@ -182,6 +182,30 @@ __device__ __forceinline__ float add_pair(unsigned w, float s, bf16)
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, s, false);
 }
 
+// 16 bytes of elements from element `at` of a buffer, zeros from the `left`th on, in moves
+// of 4 bytes (wide == 1) or of an element.
+template <class T>
+__device__ __forceinline__ u32x4 load_chunk(__amdgpu_buffer_rsrc_t r, int at, int left, int wide)
+{
+    u32x4 u;
+    if (sizeof(T) == 4 || wide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int x = e * 4 / (int)sizeof(T);
+            u[e] = __builtin_amdgcn_raw_buffer_load_b32(r, x < left ? (at + x) * (int)sizeof(T) : 0x80000000u, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned lo = __builtin_amdgcn_raw_buffer_load_b16(r, 2 * e < left ? (at + 2 * e) * 2 : 0x80000000u, 0, 0);
+            const unsigned hi =
+                __builtin_amdgcn_raw_buffer_load_b16(r, 2 * e + 1 < left ? (at + 2 * e + 1) * 2 : 0x80000000u, 0, 0);
+            u[e] = (lo & 0xffffu) | hi << 16;
+        }
+    }
+    return u;
+}
+
 // The rows of K or V of one stage into LDS, by THREADS threads (a block, or one wave on
 // its own): R rows from row `first` of n, zeros past the last and past the head's dims.
 // Chunks go straight to LDS through a buffer descriptor that ends with the last row,
@@ -207,24 +231,20 @@ struct Stage {
     __device__ __forceinline__ void issue(unsigned char* lds, int first, int tid, int wide) const
     {
         const int left = n - first;
-        const T* b = base + (long long)first * stride;
-        if (wide) {
-            const int rows = left < R ? left : R;
-            const int bytes = rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * (int)sizeof(T);
-            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, bytes, 0x00027000);
+        const int rows = left < R ? left : R;
+        const auto rsrc = buffer_of(base + (long long)first * stride,
+                                    rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * (int)sizeof(T));
+        if (wide == 2) {
             unsigned char* to = lds + (THREADS > 64 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0) * 1024;
 #pragma unroll
             for (int j = 0; j < N; ++j)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     rsrc, (__attribute__((address_space(3))) void*)(to + j * THREADS * 16), 16, off[j], 0, 0, 0);
         } else {
-#pragma unroll 1
+#pragma unroll 2
             for (int j = 0; j < N; ++j) {
                 const int c = j * THREADS + tid, r = c / S::CH, d0 = ((c % S::CH) ^ (V ? S::vswz(r) : S::kswz(r))) * S::E;
-                typename Vec<T, S::E>::type u;
-#pragma unroll
-                for (int e = 0; e < S::E; ++e) u[e] = r < left && d0 + e < dim ? b[(long long)r * stride + d0 + e] : (T)0.0f;
-                *(decltype(u)*)(lds + c * 16) = u;
+                *(u32x4*)(lds + c * 16) = load_chunk<T>(rsrc, r * (int)stride + d0, dim - d0, wide);
             }
         }
     }
@@ -243,6 +263,36 @@ __device__ __forceinline__ SeqRow seq_row(const SeqAttnArgs& p, int r, int rows,
     return {i, kvh * p.group + r - i * p.group, r < rows};
 }
 
+template <class T>
+__device__ __forceinline__ const T* row_of(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r)
+{
+    return (const T*)p.q + v.bq * p.qb + (long long)(v.q0 + r.i) * p.qt + r.head * p.qh;
+}
+
+// 16 bytes of elements from p + d0, zeros from the `left`th on; elements past the end are
+// read at the row's start instead, without a branch.
+template <class T>
+__device__ __forceinline__ u32x4 row_chunk(const T* p, int d0, int left, int wide)
+{
+    u32x4 u;
+    if (sizeof(T) == 4 || wide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int x = e * 4 / (int)sizeof(T);
+            const unsigned w = *(const unsigned*)(p + (x < left ? d0 + x : 0));
+            u[e] = x < left ? w : 0u;
+        }
+    } else {
+        const unsigned short* q = (const unsigned short*)p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned lo = q[2 * e < left ? d0 + 2 * e : 0], hi = q[2 * e + 1 < left ? d0 + 2 * e + 1 : 0];
+            u[e] = (2 * e < left ? lo : 0u) | (2 * e + 1 < left ? hi << 16 : 0u);
+        }
+    }
+    return u;
+}
+
 // The lane's q as the B operand of K Q^T: step ks holds the lane half's chunk 2 ks + h.
 template <class T, int DT>
 __device__ __forceinline__ void load_q(const SeqAttnArgs& p, const SeqView& v, const SeqRow& r,
@@ -250,21 +300,16 @@ __device__ __forceinline__ void load_q(const SeqAttnArgs& p, const SeqView& v, c
 {
     using S = SeqShape<T, DT>;
     const int h = (threadIdx.x >> 5) & 1;
-    const T* row = (const T*)p.q + v.bq * p.qb + (long long)(v.q0 + r.i) * p.qt + r.head * p.qh;
+    const auto row = row_of<T>(p, v, r);
     const bool flip = p.scale < 0.0f;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
         const int d0 = (2 * ks + h) * S::E;
         u32x4 u = {0, 0, 0, 0};
-        if (r.live && d0 < p.dim) {
-            if (p.wide) {
-                u = *(const u32x4*)(row + d0);
-            } else {
-                typename Vec<T, S::E>::type w;
-#pragma unroll
-                for (int e = 0; e < S::E; ++e) w[e] = d0 + e < p.dim ? row[d0 + e] : (T)0.0f;
-                u = __builtin_bit_cast(u32x4, w);
-            }
+        if (p.wide == 2) {
+            if (r.live && d0 < p.dim) u = *(const u32x4*)(row + d0);
+        } else if (r.live) {
+            u = row_chunk<T>(row, d0, p.dim - d0, p.wide);
         }
         if (flip) {  // c1 is positive
 #pragma unroll
@@ -287,14 +332,14 @@ __device__ __forceinline__ void load_q32(const SeqAttnArgs& p, const SeqView& v,
 #pragma unroll
         for (int x = 0; x < 8; x += 4) {
             const int d0 = (2 * ks + h) * 8 + x;
-            if (p.wide) {
-                const f32x4 u = r.live && d0 < p.dim ? *(const f32x4*)(row + d0) : (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f[x + e] = u[e] * sign;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f[x + e] = r.live && d0 + e < p.dim ? row[d0 + e] * sign : 0.0f;
+            f32x4 u = {0.f, 0.f, 0.f, 0.f};
+            if (p.wide == 2) {
+                if (r.live && d0 < p.dim) u = *(const f32x4*)(row + d0);
+            } else if (r.live) {
+                u = __builtin_bit_cast(f32x4, row_chunk<float>(row, d0, p.dim - d0, 1));
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[x + e] = u[e] * sign;
         }
         split3_x8(f, q[ks]);
     }
@@ -863,26 +908,21 @@ struct Stage32 {
     __device__ __forceinline__ void load(int first, int tid, int wide)
     {
         const int left = n - first;
-        const float* b = base + (long long)first * stride;
-        if (wide) {
-            const int rows = left < X::BK ? left : X::BK;
-            const auto rsrc = buffer_of(b, rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * 4);
+        const int rows = left < X::BK ? left : X::BK;
+        const auto rsrc =
+            buffer_of(base + (long long)first * stride, rows <= 0 ? 0 : ((rows - 1) * (int)stride + dim) * 4);
 #pragma unroll
-            for (int j = 0; j < X::N; ++j)
+        for (int j = 0; j < X::N; ++j)
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x) {
+                if (wide == 2) {
                     u[j][x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[j][x], 0, 0));
-        } else {
-#pragma unroll
-            for (int j = 0; j < X::N; ++j)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int c = j * 256 + tid, r = row_of(c), d = dim_of(c) + 4 * x + e;
-                        u[j][x][e] = c < X::CHUNKS && r < left && d < dim ? b[(long long)r * stride + d] : 0.0f;
-                    }
-        }
+                } else {
+                    const int c = j * 256 + tid, d0 = dim_of(c) + 4 * x;
+                    u[j][x] = __builtin_bit_cast(
+                        f32x4, load_chunk<float>(rsrc, row_of(c) * (int)stride + d0, c < X::CHUNKS ? dim - d0 : 0, 1));
+                }
+            }
     }
     __device__ __forceinline__ void put(unsigned char* planes, int tid) const
     {
@@ -1090,7 +1130,7 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     };
     const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
         // the other buffer's moves may still be under way
-        if (p.wide) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOVES) : "memory");
+        if (p.wide == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOVES) : "memory");
         // limits end the chunk as well: keys behind it lie in another
         f32x16 s[1][1];
         const float rc[1][1] = {{0.0f}};

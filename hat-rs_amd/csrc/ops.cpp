@@ -264,14 +264,14 @@ AttnPlan attn_plan(const hat_attention* a)
         p.chunk = 1 << 30;
         return p;
     }
-    // Chunks of keys. A block fills a CU's LDS, so 256 blocks are a round; lengths that the
-    // host does not know may leave most of a chunk empty, so they get eight rounds of
-    // smaller ones. (16 sequences of 16384 keys, 8 heads of 128: 182 us in 256 blocks, 188
-    // in 512, 200 in 1024.) Up to 128 keys a wave one chunk costs less than the join's
+    // Chunks of keys. A block fills a CU's LDS, so 256 blocks are a round; with lengths that
+    // the host does not know some stay empty, so they get two rounds. (16 sequences of
+    // 16384 keys, 8 heads of 128: 182 us in 256 blocks, 188 in 512, 200 in 1024; lengths of
+    // 8192 to 16384: 164 us in 512, 196 in 2048.) Up to 128 keys a wave one chunk costs less than the join's
     // launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
     const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
     const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
-    const long long blocks = a->cu_k || a->k_lens ? 2048 : 256, whole = 128 * split_waves(a);
+    const long long blocks = a->cu_k || a->k_lens ? 512 : 256, whole = 128 * split_waves(a);
     p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / blocks + 127) / 128 * 128));
     if (a->k_tokens <= whole) p.chunk = (int)whole;
     const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
@@ -305,6 +305,9 @@ void op_attention(const hat_attention* a, void* stream)
     if (a->k_tokens) {
         check_heads(op, "k", a->k, a->dtype);
         check_heads(op, "v", a->v, a->dtype);
+        // a stage of 64 rows lies within a buffer descriptor's 31 bits
+        check_range(op, "k's token stride", a->k.token_stride, 0, (1 << 22) - 1);
+        check_range(op, "v's token stride", a->v.token_stride, 0, (1 << 22) - 1);
         if (a->pos_q.data) {
             check_positions(op, a->pos_q);
             check_positions(op, a->pos_k);
@@ -336,12 +339,14 @@ void op_attention(const hat_attention* a, void* stream)
     p.dim = a->head_dim;
     p.q_tokens = (int)a->q_tokens, p.k_tokens = (int)a->k_tokens;
     p.causal = a->causal != 0;
-    // Rows in 16-byte chunks: aligned, a head of whole chunks, and a stage of 64 rows
-    // within a buffer descriptor's 31 bits.
     const int size = (int)element(a->dtype);
-    const long long far = (1ll << 24) / size;
-    p.wide = a->head_dim * size % 16 == 0 && aligned(a->q, a->dtype, 16) && aligned(a->k, a->dtype, 16) &&
-             aligned(a->v, a->dtype, 16) && a->k.token_stride < far && a->v.token_stride < far;
+    for (int bytes : {16, 4}) {
+        if (a->head_dim * size % bytes == 0 && aligned(a->q, a->dtype, bytes) && aligned(a->k, a->dtype, bytes) &&
+            aligned(a->v, a->dtype, bytes)) {
+            p.wide = bytes == 16 ? 2 : 1;
+            break;
+        }
+    }
     p.wide_out = a->head_dim % 4 == 0 && aligned(a->out, a->dtype, 4 * size);
     p.scale = a->scale;
     p.cap = a->cap, p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;

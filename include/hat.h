@@ -263,7 +263,7 @@ int hat_op_rotary(const hat_rotary *a, void *stream);
  * belong to no query keep what they hold.
  * causal: query i sees keys j <= i + Lk - Lq, and keys below prefix[s] (NULL:
  * none). Keys that a query does not see have no influence, whatever they hold.
- * head_dim <= 128; out may be q. workspace: hat_op_attention_workspace bytes,
+ * head_dim <= 128; k's and v's token_stride below 2^22; out may be q. workspace: hat_op_attention_workspace bytes,
  * 16-byte aligned, in use until the call's kernels end: calls (and captured
  * graphs) that may run at the same time need one each. */
 typedef struct {

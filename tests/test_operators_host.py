@@ -100,6 +100,7 @@ PQ, PK, PO = Fake(9, 4, 32), Fake(9, 2, 32), Fake(9, 4, 32, ptr=1 << 24)
     ("offsets of every sequence", (PQ, PK, PK, PO), dict(cu_q=i32(0), cu_k=i32(0))),
     ("out overlaps", (Q, K, V, Fake(2, 5, 4, 32, strides=(1280, 256, 64, 1))), {}),
     ("on top of one another", (Q, K, V, Fake(2, 5, 4, 32, strides=(640, 128, 0, 1), ptr=1 << 24)), {}),
+    ("token stride 4194304", (Q, Fake(2, 5, 2, 32, strides=(1 << 25, 1 << 22, 32, 1)), V, OUT), {}),
     ("one contiguous row", (Q, K, V, OUT), dict(workspace=Fake(2, 2, dtype="uint8"))),
     ("not a tensor of device 0", (Q, K, V, OUT), dict(workspace=Fake(2, dtype="uint8", device=-1))),
 ])
