@@ -241,7 +241,7 @@ struct Stage {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     rsrc, (__attribute__((address_space(3))) void*)(to + j * THREADS * 16), 16, off[j], 0, 0, 0);
         } else {
-#pragma unroll 2
+#pragma unroll(THREADS == 64 ? 8 : 1)  // a block's waves hide each other's waits and need the registers
             for (int j = 0; j < N; ++j) {
                 const int c = j * THREADS + tid, r = c / S::CH, d0 = ((c % S::CH) ^ (V ? S::vswz(r) : S::kswz(r))) * S::E;
                 *(u32x4*)(lds + c * 16) = load_chunk<T>(rsrc, r * (int)stride + d0, dim - d0, wide);
@@ -1108,6 +1108,7 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     const int lds = wave * X::TILE;
     constexpr int MOVES = 2 * Stage<T, DT, 32, 64, false>::N;
     const auto issue = [&](unsigned char* K, unsigned char* V, int k0) {
+        if (p.wide != 2 && k0 >= c1) return;  // nothing to wait for by count
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer's reads are done
         sk.issue(K + lds, k0, lane, p.wide);
         sv.issue(V + lds, k0, lane, p.wide);
@@ -1291,7 +1292,7 @@ SEQ_INST(hat_attnseq_f16_d2, f16, 2, 1, 2, SEQ_PLAIN, 3)
 SEQ_INST(hat_attnseq_f16_d3, f16, 3, 1, 2, SEQ_PLAIN, 2)
 SEQ_INST(hat_attnseq_f16_d4, f16, 4, 1, 2, SEQ_PLAIN, 2)
 SEQ_INST(hat_attnseq_f16_d1_bias, f16, 1, 1, 2, SEQ_BIAS, 3)
-SEQ_INST(hat_attnseq_f16_d2_bias, f16, 2, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_f16_d2_bias, f16, 2, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_f16_d3_bias, f16, 3, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_f16_d4_bias, f16, 4, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_f16_d1_cap, f16, 1, 1, 2, SEQ_CAP, 3)
@@ -1307,7 +1308,7 @@ SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 1, 2, SEQ_PLAIN, 3)
 SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 1, 2, SEQ_PLAIN, 2)
 SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 1, 2, SEQ_PLAIN, 2)
 SEQ_INST(hat_attnseq_bf16_d1_bias, bf16, 1, 1, 2, SEQ_BIAS, 3)
-SEQ_INST(hat_attnseq_bf16_d2_bias, bf16, 2, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_bf16_d2_bias, bf16, 2, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_bf16_d3_bias, bf16, 3, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_bf16_d4_bias, bf16, 4, 1, 2, SEQ_BIAS, 2)
 SEQ_INST(hat_attnseq_bf16_d1_cap, bf16, 1, 1, 2, SEQ_CAP, 3)
@@ -1332,7 +1333,7 @@ SEQ_FP_INST(hat_attnseq_f32_d1_bias, 1, 2, SEQ_BIAS, 2)
 SEQ_FP_INST(hat_attnseq_f32_d1_both, 1, 2, SEQ_BOTH, 2)
 SEQ_FP_INST(hat_attnseq_f32_d2, 2, 2, SEQ_PLAIN, 2)
 SEQ_FP_INST(hat_attnseq_f32_d2_bias, 2, 2, SEQ_BIAS, 2)
-SEQ_FP_INST(hat_attnseq_f32_d2_both, 2, 2, SEQ_BOTH, 2)
+SEQ_FP_INST(hat_attnseq_f32_d2_both, 2, 1, SEQ_BOTH, 2)
 SEQ_FP_INST(hat_attnseq_f32_d3, 3, 1, SEQ_PLAIN, 2)
 SEQ_FP_INST(hat_attnseq_f32_d3_bias, 3, 1, SEQ_BIAS, 2)
 SEQ_FP_INST(hat_attnseq_f32_d3_both, 3, 1, SEQ_BOTH, 2)
