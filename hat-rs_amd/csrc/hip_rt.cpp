@@ -51,6 +51,7 @@ const std::vector<std::string>& required_kernels()
         "hat_attnseq_f32_d1_bias", "hat_attnseq_f32_d2_bias", "hat_attnseq_f32_d3_bias", "hat_attnseq_f32_d4_bias",
         "hat_attnseq_f32_d1_both", "hat_attnseq_f32_d2_both", "hat_attnseq_f32_d3_both", "hat_attnseq_f32_d4_both",
         "hat_attnseq_f32_d1_split", "hat_attnseq_f32_d2_split", "hat_attnseq_f32_d3_split", "hat_attnseq_f32_d4_split",
+        "hat_attnseq_f32_d1_few", "hat_attnseq_f32_d2_few", "hat_attnseq_f32_d3_few", "hat_attnseq_f32_d4_few",
         "hat_attnseq_join_f32", "hat_attnseq_join_f16", "hat_attnseq_join_bf16",
         "hat_resnorm_f32_16", "hat_resnorm_f32_64", "hat_resnorm_f32_256", "hat_resnorm_f32_1024",
         "hat_resnorm_f32_64e", "hat_resnorm_f32_256e", "hat_resnorm_f32_1024e",

@@ -1050,6 +1050,77 @@ __device__ __forceinline__ long long part_row(const SeqAttnArgs& p, int slot, in
     return ((long long)slot * p.kv_heads + kvh) * ((long long)p.q_tokens * p.group) + r;
 }
 
+// A block's part of the split form: a tile of TILE rows and a chunk of keys.
+struct SplitTile {
+    SeqView v;
+    int kvh, slot, rows, prefix;
+    int row0;
+    int c0, c1;       // the chunk's keys, cut at the last row's limit
+    int least;        // the first row's limit
+};
+
+template <int TILE>
+__device__ __forceinline__ bool split_tile(const SeqAttnArgs& p, SplitTile& w)
+{
+    int tile, sq, chunk = 0, first = 0;
+    w.slot = 0;
+    if (p.cu_q) {  // b = tile slot * kv_heads + kvh, all keys in one chunk
+        w.kvh = blockIdx.x % p.kv_heads;
+        tile = blockIdx.x / p.kv_heads;
+        sq = find_sequence(p.cu_q, p.n_seq, p.q_tokens, p.group, TILE, tile, first);
+        if (sq < 0) return false;
+        tile = __builtin_amdgcn_readfirstlane(tile - first);
+    } else {  // b = (chunk slot * kv_heads + kvh) * tiles + tile
+        tile = blockIdx.x % p.tiles;
+        w.kvh = blockIdx.x / p.tiles % p.kv_heads;
+        w.slot = blockIdx.x / p.tiles / p.kv_heads;
+        if (p.cu_k) {
+            sq = find_sequence(p.cu_k, p.n_seq, p.k_tokens, 1, p.chunk, w.slot, first);
+            if (sq < 0) return false;
+            chunk = w.slot - first;
+        } else {
+            sq = w.slot / p.slots;
+            chunk = w.slot - sq * p.slots;
+        }
+    }
+    const SeqView v = w.v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    w.rows = v.lq * p.group;
+    w.row0 = tile * TILE;
+    if (w.row0 >= w.rows) return false;
+    w.prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
+    const int last = w.row0 + TILE - 1 < w.rows ? w.row0 + TILE - 1 : w.rows - 1;
+    w.least = row_limit(p, v, w.row0 / p.group, w.prefix);
+    const int end = row_limit(p, v, last / p.group, w.prefix);
+    w.c0 = chunk * p.chunk;
+    if (w.c0 >= end && chunk > 0) return false;  // no row's join asks for it; chunk 0 writes the empty rows
+    w.c1 = end - w.c0 < p.chunk ? end : w.c0 + p.chunk;
+    return true;
+}
+
+// A row of the chunk done again key by key (as in seq_finish), by one wave.
+template <class T>
+__device__ __forceinline__ void split_again(const SeqAttnArgs& p, const SplitTile& w, int r)
+{
+    const SeqView& v = w.v;
+    const int lane = threadIdx.x & 63;
+    const SeqRow sr = seq_row(p, w.row0 + r, w.rows, w.kvh);
+    int to = row_limit(p, v, sr.i, w.prefix);
+    to = to < w.c1 ? to : w.c1;
+    float m, l, oa, oc;
+    attn_row<T>(p, v, sr.i, sr.head, w.c0, to, m, l, oa, oc);
+    if (!p.part) {
+        T* out = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + sr.i) * p.ot + sr.head * p.oh;
+        if (lane < p.dim) out[lane] = (T)(oa * join_scale(l));
+        if (lane + 64 < p.dim) out[lane + 64] = (T)(oc * join_scale(l));
+    } else {
+        const long long pr = part_row(p, w.slot, w.kvh, w.row0 + r);
+        if (lane < p.dim) p.part[pr * p.dim + lane] = oa;
+        if (lane + 64 < p.dim) p.part[pr * p.dim + lane + 64] = oc;
+        if (lane == 0) p.part_ml[2 * pr] = m == -INFINITY ? -1e30f : m, p.part_ml[2 * pr + 1] = l;
+    }
+}
+
 template <class T, int DT, int W>
 __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned char* B0, unsigned char* B1,
                                                unsigned char* B2, unsigned char* B3, unsigned* P0, unsigned* P1,
@@ -1057,37 +1128,11 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
 {
     using X = SplitShape<T, DT, W>;
     constexpr int DP = 32 * DT;
-    int tile, kvh, slot = 0, sq, chunk = 0, first = 0;
-    if (p.cu_q) {  // b = tile slot * kv_heads + kvh, all keys in one chunk
-        kvh = blockIdx.x % p.kv_heads;
-        tile = blockIdx.x / p.kv_heads;
-        sq = find_sequence(p.cu_q, p.n_seq, p.q_tokens, p.group, 32, tile, first);
-        if (sq < 0) return;
-        tile = __builtin_amdgcn_readfirstlane(tile - first);
-    } else {  // b = (chunk slot * kv_heads + kvh) * tiles + tile
-        tile = blockIdx.x % p.tiles;
-        kvh = blockIdx.x / p.tiles % p.kv_heads;
-        slot = blockIdx.x / p.tiles / p.kv_heads;
-        if (p.cu_k) {
-            sq = find_sequence(p.cu_k, p.n_seq, p.k_tokens, 1, p.chunk, slot, first);
-            if (sq < 0) return;
-            chunk = slot - first;
-        } else {
-            sq = slot / p.slots;
-            chunk = slot - sq * p.slots;
-        }
-    }
-    const SeqView v = uniform(seq_view(p, __builtin_amdgcn_readfirstlane(sq)));
-    chunk = __builtin_amdgcn_readfirstlane(chunk);
-    const int rows = v.lq * p.group;
-    const int row0 = tile * 32;
-    if (row0 >= rows) return;
-    const int prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
-    const int last = row0 + 31 < rows ? row0 + 31 : rows - 1;
-    const int least = row_limit(p, v, row0 / p.group, prefix), end = row_limit(p, v, last / p.group, prefix);
-    const int c0 = chunk * p.chunk;
-    if (c0 >= end && chunk > 0) return;  // no row's join asks for it; chunk 0 writes the empty rows
-    const int c1 = end - c0 < p.chunk ? end : c0 + p.chunk;
+    SplitTile w;
+    if (!split_tile<32>(p, w)) return;
+    const SeqView& v = w.v;
+    const int kvh = w.kvh, slot = w.slot, rows = w.rows, row0 = w.row0, c0 = w.c0, c1 = w.c1, least = w.least,
+              prefix = w.prefix;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     u32x4 q[1][SeqShape<T, DT>::KS];
@@ -1225,23 +1270,234 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
         }
         if (!whole && x == 0) p.part_ml[2 * pr] = m[n], p.part_ml[2 * pr + 1] = l[n];
     }
-    for (int r = wave; r < 32; r += W) {
-        if (!((bad >> r) & 1)) continue;
-        const SeqRow sr = seq_row(p, row0 + r, rows, kvh);
-        int to = row_limit(p, v, sr.i, prefix);
-        to = to < c1 ? to : c1;
-        float rm, rl, oa, oc;
-        attn_row<T>(p, v, sr.i, sr.head, c0, to, rm, rl, oa, oc);
-        T* out = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + sr.i) * p.ot + sr.head * p.oh;
-        const long long pr = part_row(p, slot, kvh, row0 + r);
-        if (whole) {
-            if (lane < p.dim) out[lane] = (T)(oa * join_scale(rl));
-            if (lane + 64 < p.dim) out[lane + 64] = (T)(oc * join_scale(rl));
-        } else {
-            if (lane < p.dim) p.part[pr * p.dim + lane] = oa;
-            if (lane + 64 < p.dim) p.part[pr * p.dim + lane + 64] = oc;
-            if (lane == 0) p.part_ml[2 * pr] = rm == -INFINITY ? -1e30f : rm, p.part_ml[2 * pr + 1] = rl;
+    for (int r = wave; r < 32; r += W)
+        if ((bad >> r) & 1) split_again<T>(p, w, r);
+}
+
+// ---- fp32 with at most a few rows a sequence: four rows at a time on the 4 x 4 x 1 matrix
+// instruction, sixteen of them side by side. The tiles of 32 rows above spend 8192 cycles of
+// FP32 MFMA on 32 keys of 128 dims whatever the rows; this takes 2048 on 64. A wave has 64
+// keys, a lane one: K goes through LDS to the lane that owns the key (read straight from
+// memory the rows' lines were fetched eight times over: 31 us for 3 sequences of 6819 keys, 4
+// heads of 128), V comes with a dim a lane.
+//   scores: A = q, four rows, one block of lanes for each of 16 dims, picked and broadcast to
+//           the other blocks by the instruction (cbsz, abid); B = K, a dim of every lane's key.
+//   output: A = P, transposed within each four lanes so that block b holds keys 4 b .. + 3,
+//           picked the same way; B = V, a key's dims over the lanes.
+// It is then as fast as K and V arrive.
+template <int ABID>
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, 4, ABID, 0);
+}
+
+template <int X>
+__device__ __forceinline__ float quad_xor(float v)  // the lane's neighbour at lane ^ X within four
+{
+    constexpr int perm = X == 1 ? 0xb1 : X == 2 ? 0x4e : 0x1b;
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), perm, 0xf, 0xf, true));
+}
+
+// t[i] of lane j of four <- t[j] of lane i: two rounds of swaps with the neighbours.
+__device__ __forceinline__ void quad_transpose(float (&t)[4])
+{
+    const int j = threadIdx.x & 3;
+    {
+        const float a = j & 1 ? t[0] : t[1], c = j & 1 ? t[2] : t[3];
+        const float x = quad_xor<1>(a), y = quad_xor<1>(c);
+        t[0] = j & 1 ? x : t[0], t[1] = j & 1 ? t[1] : x;
+        t[2] = j & 1 ? y : t[2], t[3] = j & 1 ? t[3] : y;
+    }
+    const float a = j & 2 ? t[0] : t[2], c = j & 2 ? t[1] : t[3];
+    const float x = quad_xor<2>(a), y = quad_xor<2>(c);
+    t[0] = j & 2 ? x : t[0], t[2] = j & 2 ? t[2] : x;
+    t[1] = j & 2 ? y : t[1], t[3] = j & 2 ? t[3] : y;
+}
+
+template <int DT, int W>
+__device__ __forceinline__ void seq_few_body(const SeqAttnArgs& p, unsigned char* K, float* xo, float* ml)
+{
+    constexpr int DP = 32 * DT, SETS = (DP + 63) / 64;  // of 64 dims
+    SplitTile w;
+    if (!split_tile<4>(p, w)) return;
+    const SeqView& v = w.v;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c1 = w.c1;
+
+    float q[2 * DT];  // lane 4 b + i: row i, dim 16 j + b
+    {
+        const SeqRow r = seq_row(p, w.row0 + (lane & 3), w.rows, w.kvh);
+        const float* row = row_of<float>(p, v, r);
+        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+            const int d = 16 * j + (lane >> 2);
+            q[j] = r.live && d < p.dim ? row[d] * sign : 0.0f;
         }
+    }
+    int limit[4];
+    float slope[4], m[4], l[4];
+    unsigned pq[4][4];
+    int at[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const SeqRow sr = seq_row(p, w.row0 + r, w.rows, w.kvh);
+        limit[r] = sr.live ? row_limit(p, v, sr.i, w.prefix) : 0;
+        limit[r] = limit[r] < c1 ? limit[r] : c1;
+        const SeqBias b = seq_bias(p, v, sr, false);
+        slope[r] = b.slope, at[r] = b.at;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) pq[r][a] = b.pos[a];
+        m[r] = -1e30f, l[r] = 0.0f;
+    }
+    f32x4 o[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) o[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const float* kb = (const float*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + w.kvh * p.kh;
+    const float* vb = (const float*)p.v + v.bk * p.vb + (long long)v.k0 * p.vt + w.kvh * p.vh;
+    const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
+    const auto rows_of = [&](const float* b, long long stride, int k0) {
+        const int rows = c1 - k0 < 64 ? c1 - k0 : 64;
+        return buffer_of(b + (long long)k0 * stride, rows <= 0 ? 0 : ((rows - 1) * (int)stride + p.dim) * 4);
+    };
+    using S = SeqShape<float, DT>;
+    unsigned char* kl = K + wave * 64 * S::ROW;
+    Stage<float, DT, 64, 64, false> sk;
+    sk.init(kb, p.kt, c1, p.dim, lane);
+    int k0 = w.c0 + 64 * wave;
+    if (k0 < c1) sk.issue(kl, k0, lane, p.wide);
+    for (; k0 < c1; k0 += 64 * W) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // K has arrived
+        float vv[64][SETS];
+        const auto rv = rows_of(vb, p.vt, k0);
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+#pragma unroll
+            for (int s = 0; s < SETS; ++s)
+                vv[j][s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    rv, lane + 64 * s < p.dim ? (lane + 64 * s) * 4 : 0x80000000u, j * (int)p.vt * 4, 0));
+        f32x4 k[S::CH];
+#pragma unroll
+        for (int j = 0; j < S::CH; ++j) k[j] = *(const f32x4*)(kl + lane * S::ROW + ((j ^ S::kswz(lane)) << 4));
+        const int key = k0 + lane;
+        unsigned pk[4] = {0, 0, 0, 0};
+        if (p.pos_q) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                if (a < p.axes && key < c1) pk[a] = (unsigned)pos_k[(long long)key * p.pkt + a * p.pka] ^ 0x80000000u;
+        }
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;  // two chains
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+#define FEW_QK(B, S) S = mfma4<B>(q[j], k[4 * j + B / 4][B % 4], S);
+            FEW_QK(0, s0) FEW_QK(1, s1) FEW_QK(2, s0) FEW_QK(3, s1) FEW_QK(4, s0) FEW_QK(5, s1) FEW_QK(6, s0) FEW_QK(7, s1)
+            FEW_QK(8, s0) FEW_QK(9, s1) FEW_QK(10, s0) FEW_QK(11, s1) FEW_QK(12, s0) FEW_QK(13, s1) FEW_QK(14, s0) FEW_QK(15, s1)
+#undef FEW_QK
+        }
+        if (k0 + 64 * W < c1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+            sk.issue(kl, k0 + 64 * W, lane, p.wide);
+        }
+        float t[4];
+        bool need = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = s0[r] + s1[r];
+            if (p.cap > 0.0f)
+                x = p.cap * HAT_LOG2E * tanhf(x * fabsf(p.scale) * p.inv_cap);
+            else
+                x *= p.c1;
+            if (p.slopes) {
+                float far = fabsf((float)(at[r] - key));
+                if (p.pos_q) {
+                    unsigned u = 0;
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) u = a < p.axes ? sad(pq[r][a], pk[a], u) : u;
+                    far = (float)u;
+                }
+                x = __builtin_fmaf(-slope[r], far, x);
+            }
+            t[r] = key < limit[r] ? x : -INFINITY;
+            need |= t[r] > m[r] + 8.0f;
+        }
+        if (__any(need)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float mn = fmaxf(m[r], wave_max(t[r])), corr = fast_exp2(m[r] - mn);
+                m[r] = mn;
+                l[r] *= corr;
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) o[s][r] *= corr;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            t[r] = fast_exp2(t[r] - m[r]);
+            l[r] += t[r];
+        }
+        quad_transpose(t);  // t[i] of lane 4 b + j: row j, key 4 b + i
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+#define FEW_PV(B)                                                                                            \
+    o[s] = mfma4<B>(t[0], vv[4 * B][s], o[s]), o[s] = mfma4<B>(t[1], vv[4 * B + 1][s], o[s]),                \
+    o[s] = mfma4<B>(t[2], vv[4 * B + 2][s], o[s]), o[s] = mfma4<B>(t[3], vv[4 * B + 3][s], o[s]);
+            FEW_PV(0) FEW_PV(1) FEW_PV(2) FEW_PV(3) FEW_PV(4) FEW_PV(5) FEW_PV(6) FEW_PV(7)
+            FEW_PV(8) FEW_PV(9) FEW_PV(10) FEW_PV(11) FEW_PV(12) FEW_PV(13) FEW_PV(14) FEW_PV(15)
+#undef FEW_PV
+        }
+    }
+
+    // the waves' sums side by side
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        l[r] = wave_sum(l[r]);
+        if (lane == 0) ml[(wave * 4 + r) * 2] = m[r], ml[(wave * 4 + r) * 2 + 1] = l[r];
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) xo[(wave * 4 + r) * (64 * SETS) + 64 * s + lane] = o[s][r];
+    }
+    __syncthreads();
+    // wave x of W joins rows x, x + W, ...
+    float jo[4 / W][SETS], jm[4 / W], jl[4 / W];
+#pragma unroll
+    for (int n = 0; n < 4 / W; ++n) {
+        const int r = wave + n * W;
+        float mx = ml[r * 2];
+#pragma unroll
+        for (int x = 1; x < W; ++x) mx = fmaxf(mx, ml[(x * 4 + r) * 2]);
+        float sum = 0.0f, z = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) jo[n][s] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+            const float f = fast_exp2(ml[(x * 4 + r) * 2] - mx);
+            sum = __builtin_fmaf(f, ml[(x * 4 + r) * 2 + 1], sum);
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) jo[n][s] = __builtin_fmaf(f, xo[(x * 4 + r) * (64 * SETS) + 64 * s + lane], jo[n][s]);
+        }
+        jm[n] = mx, jl[n] = sum;
+        z = sum * 0.0f;
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) z = __builtin_fmaf(jo[n][s], 0.0f, z);
+        if (w.row0 + r >= w.rows) continue;
+        if (__any(!(z == 0.0f))) {  // as in seq_finish
+            split_again<float>(p, w, r);
+            continue;
+        }
+        const SeqRow sr = seq_row(p, w.row0 + r, w.rows, w.kvh);
+        float* out = (float*)p.o + v.bq * p.ob + (long long)(v.q0 + sr.i) * p.ot + sr.head * p.oh;
+        const long long pr = part_row(p, w.slot, w.kvh, w.row0 + r);
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+            const int d = 64 * s + lane;
+            if (d < p.dim) {
+                if (!p.part)
+                    out[d] = jo[n][s] * join_scale(jl[n]);
+                else
+                    p.part[pr * p.dim + d] = jo[n][s];
+            }
+        }
+        if (p.part && lane == 0) p.part_ml[2 * pr] = jm[n], p.part_ml[2 * pr + 1] = jl[n];
     }
 }
 
@@ -1364,6 +1620,19 @@ SPLIT_INST(hat_attnseq_f32_d1_split, float, 1, 8)
 SPLIT_INST(hat_attnseq_f32_d2_split, float, 2, 4)
 SPLIT_INST(hat_attnseq_f32_d3_split, float, 3, 2)
 SPLIT_INST(hat_attnseq_f32_d4_split, float, 4, 2)
+
+#define SEQ_FEW_INST(NAME, DT)                                                                               \
+    extern "C" __global__ __launch_bounds__(256, 1) void NAME(SeqAttnArgs p)                                 \
+    {                                                                                                        \
+        __shared__ __attribute__((aligned(16))) unsigned char K[4 * 64 * 128 * DT];                          \
+        __shared__ float xo[4 * 4 * 64 * ((DT + 1) / 2)], ml[4 * 4 * 2];                                     \
+        seq_few_body<DT, 4>(p, K, xo, ml);                                                                    \
+    }
+
+SEQ_FEW_INST(hat_attnseq_f32_d1_few, 1)
+SEQ_FEW_INST(hat_attnseq_f32_d2_few, 2)
+SEQ_FEW_INST(hat_attnseq_f32_d3_few, 3)
+SEQ_FEW_INST(hat_attnseq_f32_d4_few, 4)
 
 #define JOIN_INST(NAME, T) \
     extern "C" __global__ __launch_bounds__(256) void NAME(SeqAttnArgs p) { seq_join_body<T>(p); }

@@ -230,6 +230,7 @@ namespace {
 // How a call runs, from its sizes alone.
 struct AttnPlan {
     bool split;       // keys in chunks over blocks and waves
+    bool few;         // fp32, four rows at a time
     int tiles;        // of rows: a sequence's (batch) or all sequences' slots (packed)
     int chunk, slots; // split: keys a chunk; a sequence's chunks (batch) or all slots (packed)
     long long blocks, join_rows;  // join_rows > 0: partial results and their join
@@ -258,9 +259,13 @@ AttnPlan attn_plan(const hat_attention* a)
     // 32 whose keys the waves (and blocks) share. Times at rows.. see attnseq.hip.
     p.split = (!a->cu_q && rows <= 64) || p.blocks < 128;
     if (!p.split) return p;
-    p.tiles = (int)tiles(32);
+    // fp32 MFMA's tiles of 32 rows cost the same for one: up to eight rows go by fours (3
+    // sequences of 6819 keys, 4 heads of 128, one row: 20 us against 49).
+    p.few = a->dtype == HAT_F32 && !a->cu_q && rows <= 8;
+    const int per = p.few ? 4 : 32, waves = p.few ? 4 : split_waves(a);
+    p.tiles = (int)tiles(per);
     if (a->cu_q) {
-        p.blocks = tiles(32) * a->kv_heads;
+        p.blocks = tiles(per) * a->kv_heads;
         p.chunk = 1 << 30;
         return p;
     }
@@ -271,8 +276,8 @@ AttnPlan attn_plan(const hat_attention* a)
     // launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
     const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
     const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
-    const long long blocks = a->cu_k || a->k_lens ? 512 : 256, whole = 128 * split_waves(a);
-    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(256, (work / blocks + 127) / 128 * 128));
+    const long long blocks = a->cu_k || a->k_lens ? 512 : 256, whole = 128 * waves;
+    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(p.few ? 512 : 256, (work / blocks + 127) / 128 * 128));
     if (a->k_tokens <= whole) p.chunk = (int)whole;
     const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
     const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
@@ -364,14 +369,16 @@ void op_attention(const hat_attention* a, void* stream)
     std::string name = "hat_attnseq_" + type + "_d" + std::to_string(dim_tiles(a));
     // The bias as MFMA's starting value needs it in units of q . k: not where the scale is
     // next to nothing. fp32 has no kernel for the cap alone: its tanh is computed in full.
-    if (plan.split)
+    if (plan.few)
+        name += "_few";
+    else if (plan.split)
         name += "_split";
     else if (a->cap > 0.0f)
         name += a->slopes || a->dtype == HAT_F32 ? "_both" : "_cap";
     else if (a->slopes)
         name += p.c1 > 1e-6f ? "_bias" : "_both";
     p.fold = p.causal && !a->cu_q && plan.blocks <= 1024;
-    const int threads = plan.split ? 64 * split_waves(a) : 256;
+    const int threads = plan.split && !plan.few ? 64 * split_waves(a) : 256;
     launch(s, name.c_str(), grid_of(op, plan.blocks), 1, 1, threads, p);
     if (plan.join_rows)
         launch(s, ("hat_attnseq_join_" + type).c_str(), grid_of(op, (plan.join_rows + 3) / 4), 1, 1, 256, p);

@@ -666,6 +666,39 @@ def test_attention_far_into_a_long_cache(hl):
     assert (out[:64] == 0).all()  # sequences without keys
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [24, 33, 64, 128])
+@pytest.mark.parametrize("rows", [1, 4, 6, 8])
+def test_attention_few_queries_in_every_form(hl, kind, D, rows):
+    """Positions, a cap, a prefix, lengths on both sides, strides, unseen NaN in a seen
+    tile: one to eight rows of a key head against a few chunks of keys."""
+    hk, lk, B = 2, 1700, 3
+    lq, group = {1: (1, 1), 4: (2, 2), 6: (2, 3), 8: (8, 1)}[rows]
+    print(f"few queries in every form {kind} {D} {rows}", flush=True)
+    q, k, v = _qkv(kind, 301, (B, lq), (B, lk), hk * group, hk, D)
+    seqs = _batch(B, lq, lk)
+    _check(hl, kind, q, k, v, seqs, **_mode("grid", hk * group, lq, lk, B, 302))
+    _check(hl, kind, q, k, v, seqs, causal=True, **_mode("both grid", hk * group, lq, lk, B, 303))
+    _check(hl, kind, q, k, v, seqs, stride="odd", **_mode("negative", hk * group, lq, lk, B, 304))
+    _check(hl, kind, q, k, v, seqs, stride="heads", causal=True, prefix=torch.tensor([0, 5, 1800], dtype=torch.int32))
+    uq, uk = [lq, 0, max(1, lq - 1)], [lk, 900, 63]
+    _check(hl, kind, q, k, v, _batch(B, lq, lk, uq, uk), stride="gaps", causal=True,
+           q_lens=torch.tensor(uq, dtype=torch.int32), k_lens=torch.tensor(uk, dtype=torch.int32))
+    if lq > 1:  # the last key is seen by the last query alone
+        kb, vb = k.clone(), v.clone()
+        kb[0, -1], vb[0, -1] = math.nan, math.inf
+        qd = q.cuda()
+        out = torch.empty_like(qd)
+        need = hl.attention_workspace(qd, kb.cuda(), vb.cuda(), out, causal=True)
+        work = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+        hl.op_attention(qd, kb.cuda(), vb.cuda(), out, causal=True, workspace=work)
+        torch.cuda.synchronize()
+        assert out[0, -1].isnan().all() and torch.isfinite(out[0, :-1]).all() and torch.isfinite(out[1:]).all()
+        want, tol = _attention_want(q[0], k[0], v[0], [(slice(0, lq), slice(0, lk))], D ** -0.5, True, None, 0.0, None,
+                                    None, None, U(q.dtype))
+        assert ((out[0].cpu().double() - want).abs()[:-1] <= tol[:-1]).all()
+
+
 # Enough sequences and key heads that tiles of 128 rows fill the device: the kernels of
 # many rows, each width of a head in each of their forms.
 
