@@ -241,7 +241,7 @@ struct Stage {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     rsrc, (__attribute__((address_space(3))) void*)(to + j * THREADS * 16), 16, off[j], 0, 0, 0);
         } else {
-#pragma unroll(THREADS == 64 ? 8 : 1)  // a block's waves hide each other's waits and need the registers
+#pragma unroll 1  // the registers are needed elsewhere
             for (int j = 0; j < N; ++j) {
                 const int c = j * THREADS + tid, r = c / S::CH, d0 = ((c % S::CH) ^ (V ? S::vswz(r) : S::kswz(r))) * S::E;
                 *(u32x4*)(lds + c * 16) = load_chunk<T>(rsrc, r * (int)stride + d0, dim - d0, wide);

@@ -14,6 +14,7 @@
 
 #include "gpu.h"
 #include "kargs.h"
+#include "ops.h"
 
 namespace hat {
 
@@ -75,6 +76,176 @@ void check_close(const std::string& name, const std::vector<float>& got, const s
                  name.c_str(), worst, at, got[at], want[at], tol);
         throw Error(b);
     }
+}
+
+// ---- operators on device tensors (ops.h): host twins of the formulas in include/hat.h.
+
+// A device tensor of type HAT_F32, HAT_F16 or HAT_BF16 with values that every type holds
+// exactly: multiples of 1/64 below 2.
+struct TypedDev {
+    int dtype;
+    std::vector<double> host;
+    void* p = nullptr;
+    TypedDev(int dt, std::vector<double> v) : dtype(dt), host(std::move(v))
+    {
+        const size_t n = host.size();
+        p = Runtime::get().alloc(n * (dt == HAT_F32 ? 4 : 2));
+        if (dt == HAT_F32) {
+            std::vector<float> f(host.begin(), host.end());
+            Runtime::get().h2d(p, f.data(), n * 4);
+        } else {
+            std::vector<uint16_t> h(n);
+            for (size_t i = 0; i < n; ++i) h[i] = encode(dt, (float)host[i]);
+            Runtime::get().h2d(p, h.data(), n * 2);
+        }
+    }
+    ~TypedDev() { Runtime::get().free(p); }
+    TypedDev(const TypedDev&) = delete;
+    static uint16_t encode(int dt, float f)  // exact values only
+    {
+        uint32_t u;
+        memcpy(&u, &f, 4);
+        if (dt == HAT_BF16) return (uint16_t)(u >> 16);
+        if (f == 0.0f) return (uint16_t)(u >> 16);
+        return (uint16_t)(((u >> 16) & 0x8000) | ((((u >> 23) & 255) - 112) << 10) | ((u >> 13) & 1023));
+    }
+    std::vector<float> get() const
+    {
+        const size_t n = host.size();
+        std::vector<float> f(n);
+        Runtime::get().sync();
+        if (dtype == HAT_F32) {
+            Runtime::get().d2h(f.data(), p, n * 4);
+            return f;
+        }
+        std::vector<uint16_t> h(n);
+        Runtime::get().d2h(h.data(), p, n * 2);
+        for (size_t i = 0; i < n; ++i) {
+            if (dtype == HAT_BF16) {
+                const uint32_t u = (uint32_t)h[i] << 16;
+                memcpy(&f[i], &u, 4);
+            } else {
+                const int e = (h[i] >> 10) & 31, m = h[i] & 1023;
+                const float a = e == 31 ? INFINITY : e ? std::ldexp(1.0f + m / 1024.0f, e - 15) : std::ldexp(m / 1024.0f, -14);
+                f[i] = h[i] & 0x8000 ? -a : a;
+            }
+        }
+        return f;
+    }
+};
+
+std::vector<double> coarse(Rng& rng, size_t n)
+{
+    std::vector<double> v(n);
+    for (double& x : v) x = std::floor(rng.uni() * 127.0f) / 64.0;
+    return v;
+}
+
+// Half a step of a type on values up to 4, and what fp32 adds.
+double type_tol(int dt) { return (dt == HAT_F32 ? 0.0 : dt == HAT_F16 ? 4.0 / 2048 : 4.0 / 256) + 2e-5; }
+const char* type_tag(int dt) { return dt == HAT_F32 ? "f32" : dt == HAT_F16 ? "f16" : "bf16"; }
+
+void check_rotary(Rng& rng, int dt, int dim, int s0, int s1, bool neighbours)
+{
+    const int T = 37, heads = 3, S = s0 + s1;
+    std::vector<int> pos(2 * T);
+    for (int& x : pos) x = (int)(rng.uni() * 900);
+    TypedDev x(dt, coarse(rng, (size_t)T * heads * dim)), y(dt, std::vector<double>((size_t)T * heads * dim));
+    Dev dp(pos.size());
+    Runtime::get().h2d(dp.p, pos.data(), pos.size() * 4);
+    hat_rotary a{};
+    a.dtype = dt, a.batch = 1, a.q_heads = heads, a.head_dim = dim, a.axes = 2, a.tokens = T;
+    a.sections[0] = s0, a.sections[1] = s1, a.neighbours = neighbours, a.base = 10000.0;
+    a.pos = {(const int*)dp.p, 0, 2, 1};
+    a.q = {x.p, 0, (long long)heads * dim, dim};
+    a.q_out = {y.p, 0, (long long)heads * dim, dim};
+    op_rotary(&a, nullptr);
+    std::vector<double> want = x.host;
+    for (int t = 0; t < T; ++t)
+        for (int h = 0; h < heads; ++h)
+            for (int i = 0; i < S; ++i) {
+                const int axis = i >= s0, j = axis ? i - s0 : i;
+                const double ang = pos[2 * t + axis] * std::pow(10000.0, -(double)j / (axis ? s1 : s0));
+                const size_t b = ((size_t)t * heads + h) * dim, u = b + (neighbours ? 2 * i : i),
+                             v = b + (neighbours ? 2 * i + 1 : i + S);
+                want[u] = x.host[u] * std::cos(ang) - x.host[v] * std::sin(ang);
+                want[v] = x.host[v] * std::cos(ang) + x.host[u] * std::sin(ang);
+            }
+    check_close(std::string("hat_rotary ") + type_tag(dt), y.get(), want, type_tol(dt));
+}
+
+void check_resnorm(Rng& rng, int dt, int width)
+{
+    const int rows = 5;
+    const size_t n = (size_t)rows * width;
+    TypedDev x(dt, coarse(rng, n)), y(dt, coarse(rng, n)), g(dt, coarse(rng, width)), xo(dt, std::vector<double>(n)),
+        h(dt, std::vector<double>(n));
+    std::vector<float> w = rng.vec(width, 1.0f), b = rng.vec(width, 0.5f);
+    Dev dw(w), db(b);
+    hat_residual_norm a{};
+    a.dtype = dt, a.width = width, a.post = HAT_NORM_RMS, a.pre = HAT_NORM_LAYER, a.rows = rows, a.rows_per_gate = rows;
+    a.x = x.p, a.y = y.p, a.gate = g.p, a.x_out = xo.p, a.h = h.p;
+    a.x_stride = a.y_stride = a.gate_stride = a.x_out_stride = a.h_stride = width;
+    a.post_w = a.pre_w = dw.p, a.pre_b = db.p, a.scale = 0.5f, a.post_eps = a.pre_eps = 1e-5f;
+    op_residual_norm(&a, nullptr);
+    std::vector<double> wx(n), wh(n);
+    for (int r = 0; r < rows; ++r) {
+        double sq = 0, mean = 0, var = 0;
+        for (int c = 0; c < width; ++c) sq += y.host[(size_t)r * width + c] * y.host[(size_t)r * width + c];
+        for (int c = 0; c < width; ++c) {
+            const size_t i = (size_t)r * width + c;
+            wx[i] = x.host[i] + 0.5 * g.host[c] * (y.host[i] / std::sqrt(sq / width + 1e-5) * w[c]);
+            mean += wx[i] / width;
+        }
+        for (int c = 0; c < width; ++c) var += (wx[(size_t)r * width + c] - mean) * (wx[(size_t)r * width + c] - mean) / width;
+        for (int c = 0; c < width; ++c) {
+            const size_t i = (size_t)r * width + c;
+            wh[i] = (wx[i] - mean) / std::sqrt(var + 1e-5) * w[c] + b[c];
+        }
+    }
+    check_close(std::string("hat_resnorm ") + type_tag(dt) + " x", xo.get(), wx, type_tol(dt));
+    check_close(std::string("hat_resnorm ") + type_tag(dt) + " h", h.get(), wh, type_tol(dt));
+}
+
+// B sequences of lq queries and lk keys, causal; a sample of the rows is compared.
+void check_attention(Rng& rng, int dt, int B, int lq, int lk, int heads, int dim, bool bias, float cap)
+{
+    TypedDev q(dt, coarse(rng, (size_t)B * lq * heads * dim)), k(dt, coarse(rng, (size_t)B * lk * heads * dim)),
+        v(dt, coarse(rng, (size_t)B * lk * heads * dim)), o(dt, std::vector<double>((size_t)B * lq * heads * dim));
+    std::vector<float> slopes(heads);
+    for (int h = 0; h < heads; ++h) slopes[h] = 0.125f * h;
+    Dev ds(slopes);
+    hat_attention a{};
+    a.dtype = dt, a.n_seq = B, a.q_heads = a.kv_heads = heads, a.head_dim = dim, a.q_tokens = lq, a.k_tokens = lk;
+    const long long ts = (long long)heads * dim;
+    a.q = {q.p, lq * ts, ts, dim}, a.out = {o.p, lq * ts, ts, dim};
+    a.k = {k.p, lk * ts, ts, dim}, a.v = {v.p, lk * ts, ts, dim};
+    a.causal = 1, a.scale = 0.25f, a.cap = cap, a.slopes = bias ? ds.p : nullptr;
+    Dev ws(op_attention_workspace(&a) / 4 + 4);
+    a.workspace = ws.p, a.workspace_bytes = ws.n * 4;
+    op_attention(&a, nullptr);
+    const std::vector<float> all = o.get();
+    std::vector<float> got;
+    std::vector<double> want;
+    for (size_t row = 0; row < (size_t)B * lq * heads; row += 1 + (size_t)B * lq * heads / 300) {
+        const int h = row % heads, i = row / heads % lq, b = row / heads / lq;
+        std::vector<double> p(lk), out(dim, 0.0);
+        double sum = 0;
+        for (int j = 0; j <= i + lk - lq && j < lk; ++j) {
+            double s = 0;
+            for (int d = 0; d < dim; ++d) s += q.host[row * dim + d] * k.host[(((size_t)b * lk + j) * heads + h) * dim + d];
+            s *= 0.25;
+            if (cap > 0) s = cap * std::tanh(s / cap);
+            if (bias) s -= slopes[h] * std::fabs((double)(i + lk - lq - j));
+            p[j] = std::exp(s);
+            sum += p[j];
+        }
+        for (int j = 0; j <= i + lk - lq && j < lk; ++j)
+            for (int d = 0; d < dim; ++d) out[d] += p[j] / sum * v.host[(((size_t)b * lk + j) * heads + h) * dim + d];
+        for (int d = 0; d < dim; ++d) got.push_back(all[row * dim + d]), want.push_back(out[d]);
+    }
+    // the probabilities are rounded to the type beside the result
+    check_close(std::string("hat_attnseq ") + type_tag(dt) + " " + std::to_string(dim), got, want, type_tol(dt));
 }
 
 // mask_label (plan.rs:300-334): region of pixel (y, x) from the three bands.
@@ -1091,6 +1262,41 @@ int gpu_selftest(std::string* err)
             }
             check_close("hat_se_gate", dg.get(), want, 1e-6);
             note("hat_se_gate C 144 sq 6");
+        }
+        // ---- the operators on device tensors, every kernel by the sizes that choose it
+        for (int dt : {HAT_F32, HAT_F16, HAT_BF16}) {
+            const std::string t = type_tag(dt);
+            for (bool neighbours : {false, true}) {
+                const std::string how = neighbours ? " neighbours" : " halves";
+                check_rotary(rng, dt, 80, 16, 16, neighbours);
+                note("hat_rotary_" + t + " 16-byte moves" + how);
+                check_rotary(rng, dt, dt == HAT_F32 ? 22 : 36, dt == HAT_F32 ? 4 : 8, dt == HAT_F32 ? 6 : 8, neighbours);
+                check_rotary(rng, dt, dt == HAT_F32 ? 22 : 36, dt == HAT_F32 ? 4 : 8, dt == HAT_F32 ? 6 : 4, neighbours);
+                note("hat_rotary_" + t + " 8-byte moves" + how);
+                check_rotary(rng, dt, 33, 6, 9, neighbours);
+                note("hat_rotary_" + t + " single elements" + how);
+            }
+            for (int width : {144, 768, 1536, 4096, 16384, 1001, 3001, 9001, 1002, 3002, 9002}) {
+                check_resnorm(rng, dt, width);
+                note("hat_resnorm_" + t + " " + std::to_string(width));
+            }
+            for (int dim : {24, 64, 80, 128}) {
+                const std::string d = t + " head_dim " + std::to_string(dim);
+                check_attention(rng, dt, 32, 70, 90, 4, dim, false, 0.0f);
+                note("hat_attnseq " + d);
+                check_attention(rng, dt, 32, 70, 90, 4, dim, true, 0.0f);
+                note("hat_attnseq bias " + d);
+                check_attention(rng, dt, 32, 70, 90, 4, dim, false, 5.0f);
+                note("hat_attnseq cap " + d);
+                check_attention(rng, dt, 32, 70, 90, 4, dim, true, 5.0f);
+                note("hat_attnseq both " + d);
+                check_attention(rng, dt, 1, 20, 3000, 2, dim, true, 5.0f);
+                note("hat_attnseq split, join " + d);
+                if (dt == HAT_F32) {
+                    check_attention(rng, dt, 2, 3, 3000, 2, dim, true, 5.0f);
+                    note("hat_attnseq few, join " + d);
+                }
+            }
         }
         printf("  gpu selftest: %d checks passed\n", passed);
         fflush(stdout);
