@@ -1517,16 +1517,32 @@ __device__ __forceinline__ void seq_join_body(const SeqAttnArgs& p)
     const int limit = row_limit(p, v, row.i, p.prefix ? p.prefix[sq] : 0);
     const int n = (int)(((long long)limit + p.chunk - 1) / p.chunk);
     const int slot = p.cu_k ? v.k0 / p.chunk + sq : sq * p.slots;
+    // a lane a chunk for the weights, then the chunks' rows eight at a time
     float m = -1e30f;
     for (int c = lane; c < n; c += 64) m = fmaxf(m, p.part_ml[2 * part_row(p, slot + c, kvh, r)]);
     m = wave_max(m);
     float l = 0.0f, oa = 0.0f, oc = 0.0f;
-    for (int c = 0; c < n; ++c) {
-        const long long pr = part_row(p, slot + c, kvh, r);
-        const float f = fast_exp2(p.part_ml[2 * pr] - m);
-        l = __builtin_fmaf(f, p.part_ml[2 * pr + 1], l);
-        if (lane < p.dim) oa = __builtin_fmaf(f, p.part[pr * p.dim + lane], oa);
-        if (lane + 64 < p.dim) oc = __builtin_fmaf(f, p.part[pr * p.dim + lane + 64], oc);
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        const long long mine = 2 * part_row(p, slot + (c0 + lane < n ? c0 + lane : 0), kvh, r);
+        const float f = c0 + lane < n ? fast_exp2(p.part_ml[mine] - m) : 0.0f;
+        l += wave_sum(f * p.part_ml[mine + 1]);
+        const int here = n - c0 < 64 ? n - c0 : 64;
+        for (int x = 0; x < here; x += 8) {
+            float a[8], b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float* pr = p.part + part_row(p, slot + c0 + (x + e < here ? x + e : 0), kvh, r) * p.dim;
+                a[e] = pr[lane < p.dim ? lane : 0];
+                b[e] = pr[lane + 64 < p.dim ? lane + 64 : 0];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // a chunk past the last has the weight of none, and may hold anything
+                const float w = lane_value(f, x + e < here ? x + e : 0);
+                oa = x + e < here ? __builtin_fmaf(w, a[e], oa) : oa;
+                oc = x + e < here ? __builtin_fmaf(w, b[e], oc) : oc;
+            }
+        }
     }
     T* o = (T*)p.o + v.bq * p.ob + (long long)(v.q0 + row.i) * p.ot + row.head * p.oh;
     if (lane < p.dim) o[lane] = (T)(oa * join_scale(l));

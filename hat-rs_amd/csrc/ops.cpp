@@ -213,6 +213,8 @@ void check_attention(const hat_attention* a)
     check_range(op, "q_tokens times heads", a->q_tokens * (a->q_heads / a->kv_heads), 0, (1ll << 31) - 1024);
     if (!std::isfinite(a->scale)) throw Error("attention: scale must be finite");
     if (!(a->cap >= 0.0f) || !std::isfinite(a->cap)) throw Error("attention: cap must be 0 or positive");
+    if (a->cap > 0.0f && !(a->cap >= 1e-6f && std::fabs(a->scale) / a->cap <= 1e6f))
+        throw Error("attention: cap is next to nothing beside 1e-6 and a millionth of the scale");
     if ((a->cu_q && a->q_lens) || (a->cu_k && a->k_lens))
         throw Error("attention: a packed tensor has offsets, not lengths");
     if (a->prefix && !a->causal) throw Error("attention: a prefix belongs to the causal mask");

@@ -251,10 +251,9 @@ int hat_op_rotary(const hat_rotary *a, void *stream);
  *   s(i, j) = c tanh(scale q_i . k_j / c) - slopes[h] * distance(i, j)
  *   out_i   = sum_j e^s(i, j) v_j / sum_j e^s(i, j)
  * over the keys that query i sees; zeros where it sees none (or where every
- * weight is zero). cap 0: no tanh.
+ * weight is zero). cap 0: no tanh; else at least 1e-6, and scale / 1e6.
  * distance: |i + Lk - Lq - j| in a sequence of Lq queries and Lk keys, or with
- * positions the sum over the axes of |pos_q[i] - pos_k[j]| (differences below
- * 2^31).
+ * positions the sum over the axes of |pos_q[i] - pos_k[j]| (below 2^31).
  * Sequences: entry s of a batch, its first q_lens[s] queries and k_lens[s] keys
  * (NULL: all q_tokens, k_tokens); or, with cu_q / cu_k (n_seq + 1 rising
  * offsets), rows cu[s] .. cu[s + 1) of a packed tensor of q_tokens / k_tokens
@@ -287,7 +286,7 @@ int hat_op_attention(const hat_attention *a, void *stream);
  *   x' = x + scale * gate * Npost(y),   h = Npre(x')   (x' before its rounding)
  * N: HAT_NORM_NONE, HAT_NORM_LAYER (v - mean) / sqrt(var + eps) * w + b, or
  * HAT_NORM_RMS v / sqrt(mean v^2 + eps) * w + b; w, b fp32 [width] or NULL (ones,
- * zeros). gate: rows of `width` values, one for each rows_per_gate rows (NULL:
+ * zeros). gate: rows of `width` values, row r / rows_per_gate for row r (NULL:
  * ones). y NULL: x' = x. x_out or h may be NULL; x_out and h may be x or y. */
 enum { HAT_NORM_NONE = 0, HAT_NORM_LAYER = 1, HAT_NORM_RMS = 2 };
 typedef struct {

@@ -817,6 +817,77 @@ def test_attention_many_tiles_score_spread(hl, kind, mode):
         _check(hl, kind, q, k, v, _batch(33, 70, 400), **_mode(mode, 4, 70, 400, 33, 0))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_attention_without_keys_or_queries(hl, kind):
+    """No keys at all: zeros; no queries: no work; a batch of none."""
+    t = TYPES[kind]
+    for B, lq, hq in ((2, 3, 2), (64, 100, 4)):
+        q = torch.ones(B, lq, hq, 48, dtype=t, device="cuda")
+        k = torch.empty(B, 0, hq, 48, dtype=t, device="cuda")
+        out = torch.full_like(q, 7.0)
+        hl.op_attention(q, k, k, out, slopes=torch.ones(hq, device="cuda"),
+                        pos_q=torch.zeros(lq, 2, dtype=torch.int32, device="cuda"),
+                        pos_k=torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        assert (out == 0).all()
+        hl.op_attention(q[:, :0], q, q, out[:, :0])
+        hl.op_attention(q[:0], q[:0], q[:0], out[:0])
+
+
+def test_attention_nan_in_one_query(hl):
+    """A query with NaN is NaN and no other is, in a tile of many rows and of few."""
+    for B, lq, lk in ((64, 130, 90), (1, 5, 900)):
+        q, k, v = _qkv("bf16", 311, (B, lq), (B, lk), 2, 1, 64)
+        qb = q.clone()
+        qb[0, 2, 1, 5] = math.nan
+        out, clean = torch.empty_like(q, device="cuda"), torch.empty_like(q, device="cuda")
+        kd, vd = k.cuda(), v.cuda()
+        need = hl.attention_workspace(out, kd, vd, out.clone())
+        work = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+        hl.op_attention(qb.cuda(), kd, vd, out, workspace=work)
+        hl.op_attention(q.cuda(), kd, vd, clean, workspace=work)
+        torch.cuda.synchronize()
+        assert out[0, 2, 1].isnan().all()
+        out[0, 2, 1] = clean[0, 2, 1]
+        assert torch.equal(out, clean)
+
+
+def test_attention_on_two_streams_at_once(hl):
+    """Two calls in flight, each with a workspace of its own, against the same call alone."""
+    q, k, v = _qkv("f16", 321, (4, 1), (4, 6000), 8, 2, 128)
+    q2, k2, v2 = _qkv("f16", 322, (3, 2), (3, 5000), 8, 2, 128)
+    sets = []
+    for a in ((q, k, v), (q2, k2, v2)):
+        d = [x.cuda() for x in a]
+        out, alone = torch.empty_like(d[0]), torch.empty_like(d[0])
+        need = hl.attention_workspace(*d, out)
+        assert need > 0
+        work = torch.empty(need, dtype=torch.uint8, device="cuda")
+        hl.op_attention(*d, alone, workspace=work)
+        sets.append((d, out, alone, work, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for d, out, alone, work, s in sets:
+            hl.op_attention(*d, out, workspace=work, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for d, out, alone, work, s in sets:
+        assert torch.equal(out, alone)
+
+
+def test_attention_refuses_a_small_workspace(hl):
+    q, k, v = _qkv("f16", 331, (1, 1), (1, 6000), 8, 2, 64)
+    d = [x.cuda() for x in (q, k, v)]
+    out = torch.empty_like(d[0])
+    need = hl.attention_workspace(*d, out)
+    with pytest.raises(hl.HatError) as e:
+        hl.op_attention(*d, out)
+    assert str(need) in str(e.value)
+    with pytest.raises(hl.HatError):
+        hl.op_attention(*d, out, workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(hl.HatError):
+        hl.op_attention(*d, out, workspace=torch.empty(need + 8, dtype=torch.uint8, device="cuda")[8:])
+
+
 # ---- together ------------------------------------------------------------------------
 
 

@@ -85,6 +85,8 @@ PQ, PK, PO = Fake(9, 4, 32), Fake(9, 2, 32), Fake(9, 4, 32, ptr=1 << 24)
     ("scale must be finite", (Q, K, V, OUT), dict(scale=float("inf"))),
     ("cap must be 0 or positive", (Q, K, V, OUT), dict(cap=-1.0)),
     ("cap must be 0 or positive", (Q, K, V, OUT), dict(cap=float("nan"))),
+    ("next to nothing", (Q, K, V, OUT), dict(cap=1e-9)),
+    ("next to nothing", (Q, K, V, OUT), dict(cap=1e-3, scale=2000.0)),
     ("belongs to the causal mask", (Q, K, V, OUT), dict(prefix=i32(2))),
     ("2 contiguous values of int32", (Q, K, V, OUT), dict(prefix=i32(3), causal=True)),
     ("2 contiguous values of int32", (Q, K, V, OUT), dict(k_lens=Fake(2))),
