@@ -112,13 +112,22 @@ bool gpu_available(std::string* why)
     return true;
 }
 
+namespace {
+std::mutex g_runtime_mu;
+Runtime* g_runtime = nullptr;
+}  // namespace
+
 Runtime& Runtime::get()
 {
-    static std::mutex mu;
-    static Runtime* rt = nullptr;
-    std::lock_guard<std::mutex> g(mu);
-    if (!rt) rt = new Runtime();  // lives until the process ends
-    return *rt;
+    std::lock_guard<std::mutex> g(g_runtime_mu);
+    if (!g_runtime) g_runtime = new Runtime();  // lives until the process ends
+    return *g_runtime;
+}
+
+bool Runtime::alive()
+{
+    std::lock_guard<std::mutex> g(g_runtime_mu);
+    return g_runtime != nullptr;
 }
 
 Runtime::Runtime()
@@ -164,6 +173,7 @@ Runtime::Runtime()
     int n = 0;
     check(api_.GetDeviceCount(&n), "hipGetDeviceCount");
     if (n < 1) throw Error("no HIP device");
+    check(api_.GetDevice(&created_on_), "hipGetDevice");
     check(api_.SetDevice(0), "hipSetDevice(0)");
     check(api_.ModuleLoadData(&module_, hat_kernels_co_start), "hipModuleLoadData(gfx950 kernels)");
     for (const std::string& k : required_kernels()) {
@@ -222,9 +232,13 @@ int Runtime::cu_count() const
 
 DeviceScope::DeviceScope()
 {
-    const HipApi& api = Runtime::get().api();
-    Runtime::get().check(api.GetDevice(&before_), "hipGetDevice");
-    if (before_ != 0) Runtime::get().check(api.SetDevice(0), "hipSetDevice(0)");
+    const bool first = !Runtime::alive();
+    const Runtime& rt = Runtime::get();
+    if (first)
+        before_ = rt.created_on();
+    else
+        rt.check(rt.api().GetDevice(&before_), "hipGetDevice");
+    if (before_ != 0) rt.check(rt.api().SetDevice(0), "hipSetDevice(0)");
 }
 
 DeviceScope::~DeviceScope()

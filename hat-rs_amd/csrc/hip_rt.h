@@ -66,6 +66,10 @@ struct HipApi {
 class Runtime {
 public:
     static Runtime& get();
+    // Whether get() has been called, and the device that was current when it first was
+    // (creating the runtime makes device 0 current).
+    static bool alive();
+    int created_on() const { return created_on_; }
     const HipApi& api() const { return api_; }
     hipFunction_t fn(const char* name) const;
     const std::vector<std::string>& kernel_names() const { return names_; }
@@ -91,6 +95,7 @@ private:
     std::vector<std::string> names_;
     void* scratch_ = nullptr;
     size_t scratch_bytes_ = 0;
+    int created_on_ = 0;
 };
 
 // Makes device 0, the module's, current for a scope and the caller's again behind

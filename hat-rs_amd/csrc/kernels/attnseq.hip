@@ -3,7 +3,31 @@
 //   o_i = sum_j e^s(i, j) v_j / sum_j e^s(i, j)  over the keys j that query i sees,
 // zeros where it sees none. Every query sees the keys below a limit of its own:
 // its sequence's length, the causal edge, or the prefix where that reaches further,
-// so one number a row is the whole mask.
+// so one number a row is the whole mask, and only the stages that a limit of the wave
+// crosses compare with it. The query heads that share a key head are rows of one tile:
+// K and V are read once for all of them.
+//
+// Three forms, by rows (query, head of the group) a key head and by type; the host's
+// rules and both sides' times are at attn_plan:
+// - many rows (seq_body; fp32: seq32_body): a block of four waves, 32 rows each, walks the
+//   keys. Scores are formed transposed, S^T = K Q^T, so that a lane holds 16 scores of
+//   one row: the softmax needs one exchange with the other half of the wave, and the
+//   probabilities are MFMA's B operand for O^T += V^T P^T where they lie. V^T comes
+//   from LDS by the transposing read.
+// - few rows (seq_split_body): the keys are split over a block's waves and over blocks.
+// - fp32 with up to eight rows (seq_few_body): four rows at a time.
+//
+// What bounds the first: issue. MFMA and vector instructions take turns on a SIMD: at 16-bit
+// head_dim 128, 64 keys x 32 rows cost a wave 1024 cycles of MFMA and about 680 of the
+// softmax (32 exponentials of 8 cycles, 105 instructions of 4), 1930 measured: 53% MFMA
+// busy, LDS 53%. Two and more waves a SIMD cover each other's waits: with 64 rows a wave
+// and one wave a SIMD 787 TFLOP/s where this has 1060. The next stage's scores formed
+// under the present one's softmax gained 2% at 128 dims and lost 4% at 64: not kept.
+// Measured: bf16 16384 x 16384, 8 heads of 128 1.00-1.10 ms (1.0-1.1 PFLOP/s; the library's
+// 8192-cubed product 1.11); fp16 2 x 12 heads of 64, 4096 keys 133-149 us (700-770
+// TFLOP/s), with a bias by distance 160-169; the cap at 128 dims, causal, 2 x 16 heads, 8192
+// keys 626 us (880 TFLOP/s of the seen pairs); 256 windows of 256 tokens, 6 heads of 24,
+// bias over two axes: fp16 60-64 us, fp32 113-123.
 #include "types.h"
 
 using namespace hatk;
@@ -512,8 +536,20 @@ __device__ __forceinline__ void seq_qk(const unsigned char* K, const u32x4 (&q)[
     }
 }
 
-// The mask and the running maximum: it moves only when a score passes it by 2^8, so the
-// sums are seldom rescaled; P stays below 2^8. rc: the rows' constants (seq_start).
+// How far (log2) above 1 the largest probability is held: fp16 has 2^15 above and little
+// below, where thousands of small ones may add up (100000 of 2^-24 of the largest).
+template <class T>
+struct SeqUp {
+    static constexpr float value = 0.0f;
+};
+template <>
+struct SeqUp<f16> {
+    static constexpr float value = 6.0f;
+};
+
+// The mask and the running base, SeqUp below the largest score: it moves only when a score
+// passes it by 2^8, so the sums are seldom rescaled; P stays below 2^(8 + SeqUp). rc: the
+// rows' constants (seq_start).
 template <class T, int DT, int QT, int KT, int MODE>
 __device__ __forceinline__ void seq_max(const SeqAttnArgs& p, const unsigned* pk, int pstride, f32x16 (&s)[QT][KT],
                                         const float (&rc)[QT][KT], SeqAcc<T, DT> (&acc)[QT], const SeqBias (&bias)[QT],
@@ -548,8 +584,8 @@ __device__ __forceinline__ void seq_max(const SeqAttnArgs& p, const unsigned* pk
         }
         mx = swap_max(mx);
         if constexpr (MODE == SEQ_PLAIN || MODE == SEQ_BIAS) mx *= p.c1;
-        if (__any(mx > c.m + 8.0f)) {
-            const float mn = fmaxf(c.m, mx), corr = fast_exp2(c.m - mn);
+        if (__any(mx > c.m + (8.0f + SeqUp<T>::value))) {
+            const float mn = fmaxf(c.m, mx - SeqUp<T>::value), corr = fast_exp2(c.m - mn);
             c.m = mn;
             c.l *= corr;
 #pragma unroll
@@ -869,7 +905,10 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
 // operand enters as three bf16 parts and a product as the six terms of order <= 2 (common.h),
 // 192 cycles of MFMA for 32 x 32 x 16 where FP32 MFMA takes 512. bf16 keeps fp32's range,
 // so no operand needs a scale (two f16 parts would need one: k and v have no bound here).
-// K and V go through registers, where a block splits them once for its four waves.
+// K and V go through registers, where a block splits them once for its four waves. On FP32
+// MFMA -> here, 4 x 2048 x 2048: 8 heads of 128 550 -> 340-357 us, of 64 288 -> 201; 256
+// windows of 256 tokens, 6 heads of 24, bias over two axes: 153 -> 113-123. What is left at 24
+// dims is vector work: 13 instructions a score, 5.5 of them the probabilities' split.
 template <int DT, int KT>
 struct Seq32Shape {
     using S = SeqShape<bf16, DT>;

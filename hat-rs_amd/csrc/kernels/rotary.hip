@@ -5,7 +5,11 @@
 //
 // What bounds it: HBM, each element read and written once. The angles are shared by
 // all heads of a token, so a block computes those of its tokens once into LDS and
-// then streams the heads.
+// then streams the heads, consecutive lanes on consecutive moves of a token.
+// Measured, 57600 tokens of 12 + 12 heads in fp16: dims of 64 72-75 us (4.7-4.9 TB/s), of 80
+// with 64 turned 92 (4.8), of 72 with 64 turned 85-88 (4.5-4.7), with 56 turned in 8-byte
+// moves 90 (4.4); a large copy reaches 5.2-5.8 TB/s. A small call is its launch: 256 tokens
+// of 6 + 6 heads of 24 take 4.0 us.
 //
 // The angle is formed in double, in revolutions: position * turn keeps 2^-22 of a
 // revolution at positions of 2^31 where fp32 has lost it at 2^20, and only the

@@ -143,8 +143,8 @@ void op_rotary(const hat_rotary* a, void* stream)
     }
     check_positions(op, a->pos);
 
-    // The widest move that every row, the pairs' halves and the copied rest allow.
-    // 57600 tokens of 24 heads of 72 in f16, 28 pairs (8 bytes): see rotary.hip.
+    // The widest move that every row, the pairs' halves and the copied rest allow (57600
+    // tokens, 24 heads of 64 in fp16: 72 us in 16-byte moves, 76 in 8-byte ones).
     const int size = (int)element(a->dtype);
     const int widths[2] = {16 / size, 8 / size};
     int V = 1;
@@ -258,7 +258,9 @@ AttnPlan attn_plan(const hat_attention* a)
     p.tiles = (int)tiles(128);
     p.blocks = tiles(128) * pairs;
     // Few rows a sequence, or too few tiles of 128 to give half the CUs a block: tiles of
-    // 32 whose keys the waves (and blocks) share. Times at rows.. see attnseq.hip.
+    // 32 whose keys the waves (and blocks) share. Split against not, us: 120 tiles (3 x 2504
+    // queries, 2 heads of 80, fp16, bias over two axes) 80 and 86; 128 (2048 queries, 8 heads
+    // of 128, fp32) 318 and 274; 792 (2 x 4099, 12 heads of 64, fp16) 233 and 146.
     p.split = (!a->cu_q && rows <= 64) || p.blocks < 128;
     if (!p.split) return p;
     // fp32 MFMA's tiles of 32 rows cost the same for one: up to eight rows go by fours (3
@@ -276,10 +278,11 @@ AttnPlan attn_plan(const hat_attention* a)
     // 16384 keys, 8 heads of 128: 182 us in 256 blocks, 188 in 512, 200 in 1024; lengths of
     // 8192 to 16384: 164 us in 512, 196 in 2048.) Up to 128 keys a wave one chunk costs less than the join's
     // launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
-    const long long keys = a->cu_k ? a->k_tokens : a->k_tokens * a->n_seq;
-    const long long work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
+    const double keys = (double)a->k_tokens * (a->cu_k ? 1 : a->n_seq);
+    const double work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
     const long long blocks = a->cu_k || a->k_lens ? 512 : 256, whole = 128 * waves;
-    p.chunk = (int)std::min<long long>(1 << 30, std::max<long long>(p.few ? 512 : 256, (work / blocks + 127) / 128 * 128));
+    const long long even = (long long)std::min(work / blocks, 1e9);
+    p.chunk = (int)std::max<long long>(p.few ? 512 : 256, (even + 127) / 128 * 128);
     if (a->k_tokens <= whole) p.chunk = (int)whole;
     const long long n = (a->k_tokens + p.chunk - 1) / p.chunk;
     const long long slots = a->cu_k ? a->k_tokens / p.chunk + a->n_seq : std::max<long long>(n, 1) * a->n_seq;
@@ -379,6 +382,8 @@ void op_attention(const hat_attention* a, void* stream)
         name += a->slopes || a->dtype == HAT_F32 ? "_both" : "_cap";
     else if (a->slopes)
         name += p.c1 > 1e-6f ? "_bias" : "_both";
+    // Causal tiles in one order from the longest, or folded (attnseq.hip): 512 blocks 129 and
+    // 123 us, 792 152 and 146, 2048 629 and 680.
     p.fold = p.causal && !a->cu_q && plan.blocks <= 1024;
     const int threads = plan.split && !plan.few ? 64 * split_waves(a) : 256;
     launch(s, name.c_str(), grid_of(op, plan.blocks), 1, 1, threads, p);

@@ -888,6 +888,22 @@ def test_attention_refuses_a_small_workspace(hl):
         hl.op_attention(*d, out, workspace=torch.empty(need + 8, dtype=torch.uint8, device="cuda")[8:])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", [(33, 70, 6000, 4), (1, 2, 9000, 2)], ids=["many", "few"])
+def test_attention_many_small_probabilities(hl, kind, shape):
+    """One key far above thousands whose probabilities are 2^-15.5 of its own: subnormal
+    in fp16, a fifth of the sum together."""
+    B, lq, lk, h = shape
+    t = TYPES[kind]
+    q, k, v = torch.zeros(B, lq, h, 32, dtype=t), torch.zeros(B, lk, h, 32, dtype=t), torch.zeros(B, lk, h, 32, dtype=t)
+    q[..., 0] = 1.0
+    k[:, 7, :, 0] = 15.5
+    v[:] = 1.0
+    v[:, 7] = -1.0
+    print(f"small probabilities {kind} {shape}", flush=True)
+    _check(hl, kind, q, k, v, _batch(B, lq, lk), scale=math.log(2.0))
+
+
 # ---- together ------------------------------------------------------------------------
 
 
