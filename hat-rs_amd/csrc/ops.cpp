@@ -257,15 +257,22 @@ AttnPlan attn_plan(const hat_attention* a)
     const long long pairs = (long long)a->kv_heads * (a->cu_q ? 1 : a->n_seq);
     p.tiles = (int)tiles(128);
     p.blocks = tiles(128) * pairs;
-    // Few rows a sequence, or too few tiles of 128 to give half the CUs a block: tiles of
-    // 32 whose keys the waves (and blocks) share. Split against not, us: 120 tiles (3 x 2504
-    // queries, 2 heads of 80, fp16, bias over two axes) 80 and 86; 128 (2048 queries, 8 heads
-    // of 128, fp32) 318 and 274; 792 (2 x 4099, 12 heads of 64, fp16) 233 and 146.
-    p.split = (!a->cu_q && rows <= 64) || p.blocks < 128;
+    // Tiles of 32 rows whose keys the waves (and blocks) share, where tiles of 128 leave CUs
+    // without a block: fewer than 128 of them, or up to 256 with few rows each and keys
+    // enough to share. Split against not, us:
+    //   120 tiles (3 x 2504 queries, 2 heads of 80, fp16, bias over two axes) 80, 86; 128 (2048
+    //   queries, 8 heads of 128, fp32) 318, 274; 792 (2 x 4099, 12 heads of 64, fp16) 233, 146;
+    //   4 queries each, 8 heads of 64 / 128, fp16: 192 tiles of 256 keys 8.6, 7.5 / 10.9, 11.2, of
+    //   4096 36, 55 / 81, 112; 384 of 1024 26, 19 / 42, 35, of 4096 95, 82 / 168, 161;
+    //   1024 x 64 queries and keys, 6 heads of 32 262, 37.
+    const double keys_each = (double)a->k_tokens / (a->cu_k ? std::max(a->n_seq, 1) : 1);
+    // fp32 with up to eight rows goes by fours, whose cost follows the rows: 4 queries each, 8
+    // heads of 128, by fours against tiles of 128: 192 of 4096 keys 142, 659, 640 of 256 keys 44,
+    // 94; 6144 of 8 rows and 256 keys 673, 706 at 128 dims, 185, 113 at 32; 3 sequences
+    // of 6819 keys, 4 heads of 128, one row 20 against 49 by tiles of 32.
+    p.few = a->dtype == HAT_F32 && !a->cu_q && rows <= 8 && (dim_tiles(a) >= 3 || p.blocks <= 512);
+    p.split = p.few || p.blocks < 128 || (!a->cu_q && rows <= 64 && p.blocks <= 256 && keys_each >= 512);
     if (!p.split) return p;
-    // fp32 MFMA's tiles of 32 rows cost the same for one: up to eight rows go by fours (3
-    // sequences of 6819 keys, 4 heads of 128, one row: 20 us against 49).
-    p.few = a->dtype == HAT_F32 && !a->cu_q && rows <= 8;
     const int per = p.few ? 4 : 32, waves = p.few ? 4 : split_waves(a);
     p.tiles = (int)tiles(per);
     if (a->cu_q) {
@@ -276,8 +283,8 @@ AttnPlan attn_plan(const hat_attention* a)
     // Chunks of keys. A block fills a CU's LDS, so 256 blocks are a round; with lengths that
     // the host does not know some stay empty, so they get two rounds. (16 sequences of
     // 16384 keys, 8 heads of 128: 182 us in 256 blocks, 188 in 512, 200 in 1024; lengths of
-    // 8192 to 16384: 164 us in 512, 196 in 2048.) Up to 128 keys a wave one chunk costs less than the join's
-    // launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
+    // 8192 to 16384: 164 us in 512, 196 in 2048.) Up to 128 keys a wave one chunk costs less
+    // than the join's launch (1023 keys, 2 heads of 64: 9.4 us against 7 + 4).
     const double keys = (double)a->k_tokens * (a->cu_k ? 1 : a->n_seq);
     const double work = keys * a->kv_heads * p.tiles;  // keys times blocks that read them
     const long long blocks = a->cu_k || a->k_lens ? 512 : 256, whole = 128 * waves;

@@ -889,6 +889,21 @@ def test_attention_refuses_a_small_workspace(hl):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("shape", [(130, 1, 20, 8, 2), (70, 3, 70, 6, 2), (40, 16, 600, 4, 4), (150, 64, 64, 2, 2)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_attention_many_short_sequences(hl, kind, D, shape):
+    """Few rows each, but sequences enough to fill the device."""
+    B, lq, lk, hq, hk = shape
+    q, k, v = _qkv(kind, 341, (B, lq), (B, lk), hq, hk, D)
+    print(f"many short {kind} {D} {shape}", flush=True)
+    _check(hl, kind, q, k, v, _batch(B, lq, lk), causal=True, slopes=torch.linspace(0, 0.2, hq))
+    g = _gen(342)
+    uk = torch.randint(0, lk + 1, (B,), generator=g)
+    _check(hl, kind, q, k, v, _batch(B, lq, lk, None, uk.tolist()), k_lens=uk.to(torch.int32))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("shape", [(33, 70, 6000, 4), (1, 2, 9000, 2)], ids=["many", "few"])
 def test_attention_many_small_probabilities(hl, kind, shape):
     """One key far above thousands whose probabilities are 2^-15.5 of its own: subnormal
