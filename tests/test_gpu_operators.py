@@ -904,6 +904,53 @@ def test_attention_many_short_sequences(hl, kind, D, shape):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n", [6, 90])
+def test_attention_packed_on_one_side(hl, kind, n):
+    """A batch of queries against packed caches, and packed queries against a batch of
+    padded ones, with positions, by few sequences and by many."""
+    g = _gen(351)
+    lk = torch.randint(0, 150, (n,), generator=g)
+    cu_k = torch.cat([torch.zeros(1, dtype=torch.int64), lk.cumsum(0)]).to(torch.int32)
+    q, k, v = _qkv(kind, 352, (n, 3), (int(cu_k[-1]) + 2,), 4, 2, 64)
+    seqs = [(slice(3 * b, 3 * b + 3), slice(int(cu_k[b]), int(cu_k[b + 1]))) for b in range(n)]
+    more = dict(slopes=torch.linspace(0.0, 0.2, 4),
+                pos_q=torch.randint(0, 30, (n, 3, 2), generator=g, dtype=torch.int32),
+                pos_k=torch.randint(0, 30, (k.shape[0], 2), generator=g, dtype=torch.int32))
+    print(f"packed keys {kind} {n}", flush=True)
+    _check(hl, kind, q, k, v, seqs, causal=True, cu_k=cu_k)
+    _check(hl, kind, q, k, v, seqs, cu_k=cu_k, **more)
+    lq = torch.randint(0, 50, (n,), generator=g)
+    cu_q = torch.cat([torch.zeros(1, dtype=torch.int64), lq.cumsum(0)]).to(torch.int32)
+    q, k, v = _qkv(kind, 353, (int(cu_q[-1]) + 2,), (n, 90), 4, 2, 64)
+    uk = torch.randint(0, 91, (n,), generator=g)
+    seqs = [(slice(int(cu_q[b]), int(cu_q[b + 1])), slice(90 * b, 90 * b + int(uk[b]))) for b in range(n)]
+    print(f"packed queries {kind} {n}", flush=True)
+    _check(hl, kind, q, k, v, seqs, causal=True, cu_q=cu_q, k_lens=uk.to(torch.int32))
+    more = dict(slopes=torch.linspace(0.0, 0.2, 4),
+                pos_q=torch.randint(0, 30, (q.shape[0], 2), generator=g, dtype=torch.int32),
+                pos_k=torch.randint(0, 30, (n, 90, 2), generator=g, dtype=torch.int32))
+    _check(hl, kind, q, k, v, seqs, cap=9.0, cu_q=cu_q, k_lens=uk.to(torch.int32), **more)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_attention_offsets_out_of_range_are_clamped(hl, kind):
+    """Offsets and lengths that point outside the tensors read and write nothing there."""
+    q, k, v = _qkv(kind, 361, (300,), (300,), 32, 32, 32)
+    qd, kd, vd = q.cuda(), k.cuda(), v.cuda()
+    guard = torch.full((340, 32, 32), 55.0, dtype=q.dtype, device="cuda")
+    out = guard[20:320]
+    cu = torch.tensor([-50, 100, 100, 299, 100000, 2 ** 31 - 1], dtype=torch.int32).cuda()
+    hl.op_attention(qd, kd, vd, out, cu_q=cu, cu_k=cu, causal=True)
+    torch.cuda.synchronize()
+    assert (guard[:20] == 55.0).all() and (guard[320:] == 55.0).all()
+    good = torch.tensor([0, 100, 100, 299, 300, 300], dtype=torch.int32).cuda()
+    want = torch.empty_like(qd)
+    hl.op_attention(qd, kd, vd, want, cu_q=good, cu_k=good, causal=True)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("shape", [(33, 70, 6000, 4), (1, 2, 9000, 2)], ids=["many", "few"])
 def test_attention_many_small_probabilities(hl, kind, shape):
     """One key far above thousands whose probabilities are 2^-15.5 of its own: subnormal
