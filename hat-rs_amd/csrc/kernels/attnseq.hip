@@ -27,7 +27,7 @@
 // 8192-cubed product 1.11); fp16 2 x 12 heads of 64, 4096 keys 133-149 us (700-770
 // TFLOP/s), with a bias by distance 160-169; the cap at 128 dims, causal, 2 x 16 heads, 8192
 // keys 626 us (880 TFLOP/s of the seen pairs); 256 windows of 256 tokens, 6 heads of 24,
-// bias over two axes: fp16 60-64 us, fp32 113-123.
+// bias over two axes: fp16 60-64 us, fp32 110-123.
 #include "types.h"
 
 using namespace hatk;
@@ -506,12 +506,11 @@ __device__ __forceinline__ void seq_scores(const SeqAttnArgs& p, const SeqBias& 
         index_bias(b, s, k0);
 }
 
-// S^T = K Q^T of KT x 32 keys and QT x 32 rows (A = 32 keys, B = the wave's q), so that
+// S^T = K Q^T of KT x 32 keys and 32 rows (A = 32 keys, B = the wave's q), so that
 // a lane holds 16 scores of one row and, as probabilities, the B operand of O^T += V^T P^T
 // without a move. s: where it starts from.
-template <class T, int DT, int QT, int KT>
-__device__ __forceinline__ void seq_qk(const unsigned char* K, const u32x4 (&q)[QT][SeqShape<T, DT>::KS],
-                                       f32x16 (&s)[QT][KT])
+template <class T, int DT, int KT>
+__device__ __forceinline__ void seq_qk(const unsigned char* K, const u32x4 (&q)[SeqShape<T, DT>::KS], f32x16 (&s)[KT])
 {
     using S = SeqShape<T, DT>;
     const int lane = threadIdx.x & 63, ql = lane & 31, h = lane >> 5;
@@ -522,15 +521,11 @@ __device__ __forceinline__ void seq_qk(const unsigned char* K, const u32x4 (&q)[
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
             const u32x4 a = *(const u32x4*)(K + at + kt * 32 * S::ROW);
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[t][kt] = mfma32(__uint_as_float(a[e]), __uint_as_float(q[t][ks][e]), s[t][kt]);
-                } else {
-                    s[t][kt] = mma16(a, q[t][ks], s[t][kt], T());
-                }
+                for (int e = 0; e < 4; ++e) s[kt] = mfma32(__uint_as_float(a[e]), __uint_as_float(q[ks][e]), s[kt]);
+            } else {
+                s[kt] = mma16(a, q[ks], s[kt], T());
             }
         }
     }
@@ -550,77 +545,69 @@ struct SeqUp<f16> {
 // The mask and the running base, SeqUp below the largest score: it moves only when a score
 // passes it by 2^8, so the sums are seldom rescaled; P stays below 2^(8 + SeqUp). rc: the
 // rows' constants (seq_start).
-template <class T, int DT, int QT, int KT, int MODE>
-__device__ __forceinline__ void seq_max(const SeqAttnArgs& p, const unsigned* pk, int pstride, f32x16 (&s)[QT][KT],
-                                        const float (&rc)[QT][KT], SeqAcc<T, DT> (&acc)[QT], const SeqBias (&bias)[QT],
-                                        const int (&limit)[QT], int k0, bool masked)
+template <class T, int DT, int KT, int MODE>
+__device__ __forceinline__ void seq_max(const SeqAttnArgs& p, const unsigned* pk, int pstride, f32x16 (&s)[KT],
+                                        const float (&rc)[KT], SeqAcc<T, DT>& c, const SeqBias& bias, int limit, int k0,
+                                        bool masked)
 {
     const int h = (threadIdx.x >> 5) & 1;
     const float a = p.cap * HAT_LOG2E;
+    float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        SeqAcc<T, DT>& c = acc[t];
-        float mx = -INFINITY;
+    for (int kt = 0; kt < KT; ++kt) {
+        f32x16& x = s[kt];
+        if constexpr (MODE == SEQ_BOTH) seq_scores<T>(p, bias, x, k0 + 32 * kt, pk + 32 * kt, pstride);
+        if constexpr (MODE == SEQ_CAP) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            f32x16& x = s[t][kt];
-            if constexpr (MODE == SEQ_BOTH) seq_scores<T>(p, bias[t], x, k0 + 32 * kt, pk + 32 * kt, pstride);
-            if constexpr (MODE == SEQ_CAP) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_rcpf(fast_exp2(x[r] * p.c1) + 1.0f);
-            }
-            if (masked) {
-                const float out = MODE == SEQ_CAP ? INFINITY : -INFINITY;
-                const int left = limit[t] - k0 - 32 * kt - 4 * h;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + (r & 3) < left ? x[r] : out;
-            }
-            float m = x[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) m = MODE == SEQ_CAP ? fminf(m, x[r]) : fmaxf(m, x[r]);
-            if constexpr (MODE == SEQ_CAP) m = __builtin_fmaf(-2.0f * a, m, a);
-            if constexpr (MODE == SEQ_BIAS) m += rc[t][kt];
-            mx = fmaxf(mx, m);
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_rcpf(fast_exp2(x[r] * p.c1) + 1.0f);
         }
-        mx = swap_max(mx);
-        if constexpr (MODE == SEQ_PLAIN || MODE == SEQ_BIAS) mx *= p.c1;
-        if (__any(mx > c.m + (8.0f + SeqUp<T>::value))) {
-            const float mn = fmaxf(c.m, mx - SeqUp<T>::value), corr = fast_exp2(c.m - mn);
-            c.m = mn;
-            c.l *= corr;
+        if (masked) {
+            const float out = MODE == SEQ_CAP ? INFINITY : -INFINITY;
+            const int left = limit - k0 - 32 * kt - 4 * h;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) c.o[d][r] *= corr;
+            for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + (r & 3) < left ? x[r] : out;
         }
+        float m = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = MODE == SEQ_CAP ? fminf(m, x[r]) : fmaxf(m, x[r]);
+        if constexpr (MODE == SEQ_CAP) m = __builtin_fmaf(-2.0f * a, m, a);
+        if constexpr (MODE == SEQ_BIAS) m += rc[kt];
+        mx = fmaxf(mx, m);
+    }
+    mx = swap_max(mx);
+    if constexpr (MODE == SEQ_PLAIN || MODE == SEQ_BIAS) mx *= p.c1;
+    if (__any(mx > c.m + (8.0f + SeqUp<T>::value))) {
+        const float mn = fmaxf(c.m, mx - SeqUp<T>::value), corr = fast_exp2(c.m - mn);
+        c.m = mn;
+        c.l *= corr;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) c.o[d][r] *= corr;
     }
 }
 
 // The probabilities 2^(s - m), in place (fp32) or packed for the product (16-bit types).
-template <class T, int DT, int QT, int KT, int MODE>
-__device__ __forceinline__ void seq_exp(const SeqAttnArgs& p, f32x16 (&s)[QT][KT], const float (&rc)[QT][KT],
-                                        SeqAcc<T, DT> (&acc)[QT], u32x4 (&pb)[QT][KT][2])
+template <class T, int DT, int KT, int MODE>
+__device__ __forceinline__ void seq_exp(const SeqAttnArgs& p, f32x16 (&s)[KT], const float (&rc)[KT], SeqAcc<T, DT>& c,
+                                        u32x4 (&pb)[KT][2])
 {
     const float a = p.cap * HAT_LOG2E;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        SeqAcc<T, DT>& c = acc[t];
+    for (int kt = 0; kt < KT; ++kt) {
+        const float f = MODE == SEQ_CAP ? -2.0f * a : p.c1;
+        const float m = MODE == SEQ_CAP ? a - c.m : MODE == SEQ_BIAS ? __builtin_fmaf(rc[kt], p.c1, -c.m) : -c.m;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const float f = MODE == SEQ_CAP ? -2.0f * a : p.c1;
-            const float m = MODE == SEQ_CAP ? a - c.m : MODE == SEQ_BIAS ? __builtin_fmaf(rc[t][kt], p.c1, -c.m) : -c.m;
+        for (int r = 0; r < 16; ++r) {
+            s[kt][r] = fast_exp2(MODE == SEQ_BOTH ? s[kt][r] + m : __builtin_fmaf(s[kt][r], f, m));
+            if constexpr (sizeof(T) == 4) c.l += s[kt][r];
+        }
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[t][kt][r] = fast_exp2(MODE == SEQ_BOTH ? s[t][kt][r] + m : __builtin_fmaf(s[t][kt][r], f, m));
-                if constexpr (sizeof(T) == 4) c.l += s[t][kt][r];
-            }
-            if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const unsigned w = pack16(s[t][kt][r], s[t][kt][r + 1], T());
-                    pb[t][kt][r >> 3][(r & 7) >> 1] = w;
-                    c.l = add_pair(w, c.l, T());
-                }
+            for (int r = 0; r < 16; r += 2) {
+                const unsigned w = pack16(s[kt][r], s[kt][r + 1], T());
+                pb[kt][r >> 3][(r & 7) >> 1] = w;
+                c.l = add_pair(w, c.l, T());
             }
         }
     }
@@ -640,9 +627,9 @@ __device__ __forceinline__ u32x4 read_v(const unsigned char* at, int step)
 
 // O^T += V^T P^T. With MFMA's key order within 16 (lane half h, slot j: keys 4 h + j,
 // then 8 + 4 h + j - 4) V's 16-bit operand is two transposed reads of four keys each.
-template <class T, int DT, int QT, int KT>
-__device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)[QT][KT], const u32x4 (&pb)[QT][KT][2],
-                                       SeqAcc<T, DT> (&acc)[QT])
+template <class T, int DT, int KT>
+__device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)[KT], const u32x4 (&pb)[KT][2],
+                                       SeqAcc<T, DT>& c)
 {
     using S = SeqShape<T, DT>;
     const int lane = threadIdx.x & 63, ql = lane & 31, h = lane >> 5;
@@ -655,8 +642,7 @@ __device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const float a = *(const float*)(row + d * 128);
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) acc[t].o[d] = mfma32(a, s[t][kt][r], acc[t].o[d]);
+                    c.o[d] = mfma32(a, s[kt][r], c.o[d]);
                 }
             }
     } else {
@@ -670,9 +656,7 @@ __device__ __forceinline__ void seq_pv(const unsigned char* V, const f32x16 (&s)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const u32x4 a = read_v(V + row + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW, 8 * S::ROW);
-#pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        acc[t].o[d] = mma16(a, pb[t][kt][st], acc[t].o[d], T());
+                    c.o[d] = mma16(a, pb[kt][st], c.o[d], T());
                 }
     }
 }
@@ -723,7 +707,7 @@ __device__ __forceinline__ SeqView uniform(const SeqView& v)
     return w;
 }
 
-// A block's tile of 128 QT rows, and its waves' shares: 32 QT rows each.
+// A block's tile of 128 rows, and its waves' shares: 32 rows each.
 struct SeqTile {
     SeqView v;
     int kvh, rows, prefix;
@@ -733,10 +717,9 @@ struct SeqTile {
     int at0, at1;     // i + Lk - Lq of its first and last row
 };
 
-template <int QT>
 __device__ __forceinline__ bool seq_tile(const SeqAttnArgs& p, SeqTile& w)
 {
-    constexpr int BQ = 128 * QT;
+    constexpr int BQ = 128;
     const int pairs = p.cu_q ? p.kv_heads : p.kv_heads * p.n_seq;
     const int pair = blockIdx.x % pairs;
     int tile = blockIdx.x / pairs, sq;
@@ -763,16 +746,16 @@ __device__ __forceinline__ bool seq_tile(const SeqAttnArgs& p, SeqTile& w)
         tile = p.fold && tile >= half ? tile - half : tiles - 1 - tile;
     }
     w.prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[v.s]) : 0;
-    w.row0 = tile * BQ + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32 * QT;
+    w.row0 = tile * BQ + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
     const int block_last = tile * BQ + BQ - 1 < w.rows ? tile * BQ + BQ - 1 : w.rows - 1;
     w.end = row_limit(p, v, block_last / p.group, w.prefix);
     w.least = 0x7fffffff, w.most = 0;
     if (w.row0 < w.rows) {
         w.least = row_limit(p, v, w.row0 / p.group, w.prefix);
-        const int last = w.row0 + 32 * QT - 1 < w.rows ? w.row0 + 32 * QT - 1 : w.rows - 1;
+        const int last = w.row0 + 31 < w.rows ? w.row0 + 31 : w.rows - 1;
         w.most = row_limit(p, v, last / p.group, w.prefix);
     }
-    w.at0 = w.row0 / p.group + v.lk - v.lq, w.at1 = (w.row0 + 32 * QT - 1) / p.group + v.lk - v.lq;
+    w.at0 = w.row0 / p.group + v.lk - v.lq, w.at1 = (w.row0 + 31) / p.group + v.lk - v.lq;
     return true;
 }
 
@@ -823,30 +806,25 @@ __device__ __forceinline__ void seq_finish(const SeqAttnArgs& p, const SeqTile& 
     }
 }
 
-// ---- many rows: a block of four waves, QT x 32 rows each, walks the keys in stages of
+// ---- many rows: a block of four waves, 32 rows each, walks the keys in stages of
 // KT x 32, two in LDS: the next one's copy runs under the present one's products.
-template <class T, int DT, int QT, int KT, int MODE>
+template <class T, int DT, int KT, int MODE>
 __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0, unsigned char* K1, unsigned char* V0,
                                          unsigned char* V1, unsigned* P0, unsigned* P1)
 {
     constexpr int BK = 32 * KT;
     SeqTile w;
-    if (!seq_tile<QT>(p, w)) return;
+    if (!seq_tile(p, w)) return;
     const SeqView& v = w.v;
     const int tid = threadIdx.x, lane = tid & 63;
-    u32x4 q[QT][SeqShape<T, DT>::KS];
-    SeqAcc<T, DT> acc[QT];
-    SeqBias bias[QT];
-    SeqRow row[QT];
-    int limit[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        row[t] = seq_row(p, w.row0 + 32 * t + (lane & 31), w.rows, w.kvh);
-        load_q<T, DT>(p, v, row[t], q[t]);
-        limit[t] = row[t].live ? row_limit(p, v, row[t].i, w.prefix) : 0x7fffffff;
-        if constexpr (MODE == SEQ_BIAS || MODE == SEQ_BOTH) bias[t] = seq_bias(p, v, row[t], MODE == SEQ_BIAS);
-        acc[t].init();
-    }
+    const SeqRow row = seq_row(p, w.row0 + (lane & 31), w.rows, w.kvh);
+    const int limit = row.live ? row_limit(p, v, row.i, w.prefix) : 0x7fffffff;
+    u32x4 q[SeqShape<T, DT>::KS];
+    load_q<T, DT>(p, v, row, q);
+    SeqBias bias;
+    if constexpr (MODE == SEQ_BIAS || MODE == SEQ_BOTH) bias = seq_bias(p, v, row, MODE == SEQ_BIAS);
+    SeqAcc<T, DT> acc;
+    acc.init();
 
     Stage<T, DT, BK, 256, false> sk;
     Stage<T, DT, BK, 256, true> sv;
@@ -855,18 +833,16 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
     const int* pos_k = p.pos_k + v.bk * p.pkb + (long long)v.k0 * p.pkt;
     const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
         if (k0 >= w.most) return;
-        f32x16 s[QT][KT];
-        float rc[QT][KT];
-        u32x4 pb[QT][KT][2];
+        f32x16 s[KT];
+        float rc[KT];
+        u32x4 pb[KT][2];
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-                rc[t][kt] = seq_start<MODE>(p, bias[t], s[t][kt], k0 + 32 * kt, P + 32 * kt, BK, w.at0, w.at1);
-        seq_qk<T, DT, QT, KT>(K, q, s);
-        seq_max<T, DT, QT, KT, MODE>(p, P, BK, s, rc, acc, bias, limit, k0, k0 + BK > w.least);
-        seq_exp<T, DT, QT, KT, MODE>(p, s, rc, acc, pb);
-        seq_pv<T, DT, QT, KT>(V, s, pb, acc);
+        for (int kt = 0; kt < KT; ++kt)
+            rc[kt] = seq_start<MODE>(p, bias, s[kt], k0 + 32 * kt, P + 32 * kt, BK, w.at0, w.at1);
+        seq_qk<T, DT, KT>(K, q, s);
+        seq_max<T, DT, KT, MODE>(p, P, BK, s, rc, acc, bias, limit, k0, k0 + BK > w.least);
+        seq_exp<T, DT, KT, MODE>(p, s, rc, acc, pb);
+        seq_pv<T, DT, KT>(V, s, pb, acc);
     };
     // The positions of a stage's keys, one a thread: read with the stage's copies, put into
     // LDS behind the present stage's products.
@@ -897,8 +873,7 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
             __syncthreads();
         }
     }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) seq_finish<T, DT>(p, w, row[t], w.row0 + 32 * t, acc[t]);
+    seq_finish<T, DT>(p, w, row, w.row0, acc);
 }
 
 // ---- fp32 with many rows: the same walk on the BF16 matrix path at fp32 accuracy. Every
@@ -907,7 +882,7 @@ __device__ __forceinline__ void seq_body(const SeqAttnArgs& p, unsigned char* K0
 // so no operand needs a scale (two f16 parts would need one: k and v have no bound here).
 // K and V go through registers, where a block splits them once for its four waves. On FP32
 // MFMA -> here, 4 x 2048 x 2048: 8 heads of 128 550 -> 340-357 us, of 64 288 -> 201; 256
-// windows of 256 tokens, 6 heads of 24, bias over two axes: 153 -> 113-123. What is left at 24
+// windows of 256 tokens, 6 heads of 24, bias over two axes: 153 -> 110-123. What is left at 24
 // dims is vector work: 13 instructions a score, 5.5 of them the probabilities' split.
 template <int DT, int KT>
 struct Seq32Shape {
@@ -994,17 +969,17 @@ __device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* 
     using X = Seq32Shape<DT, KT>;
     using S = SeqShape<bf16, DT>;
     SeqTile w;
-    if (!seq_tile<1>(p, w)) return;
+    if (!seq_tile(p, w)) return;
     const SeqView& v = w.v;
     const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
     const SeqRow row = seq_row(p, w.row0 + ql, w.rows, w.kvh);
     u32x4 q[S::KS][3];
     load_q32<DT>(p, v, row, q);
-    SeqAcc<float, DT> acc[1];
-    acc[0].init();
-    SeqBias bias[1];
-    if constexpr (MODE != SEQ_PLAIN) bias[0] = seq_bias(p, v, row, MODE == SEQ_BIAS);
-    const int limit[1] = {row.live ? row_limit(p, v, row.i, w.prefix) : 0x7fffffff};
+    SeqAcc<float, DT> acc;
+    acc.init();
+    SeqBias bias;
+    if constexpr (MODE != SEQ_PLAIN) bias = seq_bias(p, v, row, MODE == SEQ_BIAS);
+    const int limit = row.live ? row_limit(p, v, row.i, w.prefix) : 0x7fffffff;
     Stage32<DT, KT, false> sk;
     Stage32<DT, KT, true> sv;
     sk.init((const float*)p.k + v.bk * p.kb + (long long)v.k0 * p.kt + w.kvh * p.kh, p.kt, v.lk, p.dim, tid);
@@ -1026,11 +1001,11 @@ __device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* 
         __syncthreads();
         load(k0 + X::BK);  // past the last key: zeros
         if (k0 < w.most) {
-            f32x16 s[1][KT];
-            float rc[1][KT];
+            f32x16 s[KT];
+            float rc[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
-                rc[0][kt] = seq_start<MODE>(p, bias[0], s[0][kt], k0 + 32 * kt, P + 32 * kt, X::BK, w.at0, w.at1);
+                rc[kt] = seq_start<MODE>(p, bias, s[kt], k0 + 32 * kt, P + 32 * kt, X::BK, w.at0, w.at1);
 #pragma unroll
             for (int ks = 0; ks < S::KS; ++ks) {
                 const int at = ql * S::ROW + (((2 * ks + h) ^ S::kswz(ql)) << 4);
@@ -1039,12 +1014,12 @@ __device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* 
                     u32x4 a[3];
 #pragma unroll
                     for (int pl = 0; pl < 3; ++pl) a[pl] = *(const u32x4*)(Kp + pl * X::PLANE + at + kt * 32 * S::ROW);
-                    s[0][kt] = mfma6(a, q[ks], s[0][kt]);
+                    s[kt] = mfma6(a, q[ks], s[kt]);
                 }
             }
-            seq_max<float, DT, 1, KT, MODE>(p, P, X::BK, s, rc, acc, bias, limit, k0, k0 + X::BK > w.least);
-            u32x4 none[1][KT][2];
-            seq_exp<float, DT, 1, KT, MODE>(p, s, rc, acc, none);
+            seq_max<float, DT, KT, MODE>(p, P, X::BK, s, rc, acc, bias, limit, k0, k0 + X::BK > w.least);
+            u32x4 none[KT][2];
+            seq_exp<float, DT, KT, MODE>(p, s, rc, acc, none);
             const int x = lane & 15, kr = 4 * h + (x >> 2);
             const int vrow = kr * S::ROW + (x & 1) * 8;
             const int lc = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1), vsw = S::vswz(kr);
@@ -1054,7 +1029,7 @@ __device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* 
                 for (int st = 0; st < 2; ++st) {
                     float f[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = s[0][kt][8 * st + j];
+                    for (int j = 0; j < 8; ++j) f[j] = s[kt][8 * st + j];
                     u32x4 b[3];
                     split3_x8(f, b);
 #pragma unroll
@@ -1064,13 +1039,13 @@ __device__ __forceinline__ void seq32_body(const SeqAttnArgs& p, unsigned char* 
                         for (int pl = 0; pl < 3; ++pl)
                             a[pl] = read_v(Vp + pl * X::PLANE + vrow + ((lc + 4 * d) ^ vsw) * 16 + (32 * kt + 16 * st) * S::ROW,
                                            8 * S::ROW);
-                        acc[0].o[d] = mfma6(a, b, acc[0].o[d]);
+                        acc.o[d] = mfma6(a, b, acc.o[d]);
                     }
                 }
         }
         __syncthreads();  // the stage has been read
     }
-    seq_finish<float, DT>(p, w, row, w.row0, acc[0]);
+    seq_finish<float, DT>(p, w, row, w.row0, acc);
 }
 
 // ---- few rows a sequence (a token each, say) against many keys: the keys go over blocks
@@ -1177,15 +1152,14 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
               prefix = w.prefix;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    u32x4 q[1][SeqShape<T, DT>::KS];
-    SeqAcc<T, DT> acc[1];
-    SeqBias bias[1];
-    int limit[1];
+    u32x4 q[SeqShape<T, DT>::KS];
     const SeqRow row = seq_row(p, row0 + (lane & 31), rows, kvh);
-    load_q<T, DT>(p, v, row, q[0]);
-    limit[0] = row.live ? row_limit(p, v, row.i, prefix) : 0x7fffffff;
-    bias[0] = seq_bias(p, v, row, false);
-    acc[0].init();
+    load_q<T, DT>(p, v, row, q);
+    int limit = row.live ? row_limit(p, v, row.i, prefix) : 0x7fffffff;
+    limit = limit < c1 ? limit : c1;  // keys behind the chunk lie in another
+    const SeqBias bias = seq_bias(p, v, row, false);
+    SeqAcc<T, DT> c;
+    c.init();
 
     Stage<T, DT, 32, 64, false> sk;
     Stage<T, DT, 32, 64, true> sv;
@@ -1219,18 +1193,16 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     const auto stage = [&](const unsigned char* K, const unsigned char* V, const unsigned* P, int k0) {
         // the other buffer's moves may still be under way
         if (WIDE) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOVES) : "memory");
-        // limits end the chunk as well: keys behind it lie in another
-        f32x16 s[1][1];
-        const float rc[1][1] = {{0.0f}};
-        u32x4 pb[1][1][2];
+        f32x16 s[1];
+        const float rc[1] = {0.0f};
+        u32x4 pb[1][2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[0][0][r] = 0.0f;
-        seq_qk<T, DT, 1, 1>(K + lds, q, s);
-        seq_max<T, DT, 1, 1, SEQ_BOTH>(p, P + wave * 128, 32, s, rc, acc, bias, limit, k0, k0 + 32 > least || k0 + 32 > c1);
-        seq_exp<T, DT, 1, 1, SEQ_BOTH>(p, s, rc, acc, pb);
-        seq_pv<T, DT, 1, 1>(V + lds, s, pb, acc);
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.0f;
+        seq_qk<T, DT, 1>(K + lds, q, s);
+        seq_max<T, DT, 1, SEQ_BOTH>(p, P + wave * 128, 32, s, rc, c, bias, limit, k0, k0 + 32 > least || k0 + 32 > c1);
+        seq_exp<T, DT, 1, SEQ_BOTH>(p, s, rc, c, pb);
+        seq_pv<T, DT, 1>(V + lds, s, pb, c);
     };
-    limit[0] = limit[0] < c1 ? limit[0] : c1;
     int k0 = c0 + 32 * wave;
     read_pos(k0);
     issue(B0, B2, k0);
@@ -1249,7 +1221,6 @@ __device__ __forceinline__ void seq_split_body(const SeqAttnArgs& p, unsigned ch
     }
 
     // the waves' sums side by side: 32 dims of each row in a buffer
-    SeqAcc<T, DT>& c = acc[0];
     c.l = swap_sum(c.l);
     if (tid == 0) *flags = 0;
     __syncthreads();  // every wave is through its stages, and its moves have arrived
@@ -1591,48 +1562,48 @@ __device__ __forceinline__ void seq_join_body(const SeqAttnArgs& p)
     if (lane + 64 < p.dim) o[lane + 64] = (T)(oc * join_scale(l));
 }
 
-#define SEQ_INST(NAME, T, DT, QT, KT, MODE, WPS)                                                             \
+#define SEQ_INST(NAME, T, DT, KT, MODE, WPS)                                                                 \
     extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
     {                                                                                                        \
         constexpr int B = 32 * KT * SeqShape<T, DT>::ROW;                                                    \
         constexpr int PB = MODE == SEQ_BIAS || MODE == SEQ_BOTH ? 128 * KT : 4;                              \
         __shared__ __attribute__((aligned(16))) unsigned char K0[B], K1[B], V0[B], V1[B];                    \
         __shared__ __attribute__((aligned(16))) unsigned P0[PB], P1[PB];                                     \
-        seq_body<T, DT, QT, KT, MODE>(p, K0, K1, V0, V1, P0, P1);                                            \
+        seq_body<T, DT, KT, MODE>(p, K0, K1, V0, V1, P0, P1);                                                \
     }
 
-SEQ_INST(hat_attnseq_f16_d1, f16, 1, 1, 2, SEQ_PLAIN, 3)
-SEQ_INST(hat_attnseq_f16_d2, f16, 2, 1, 2, SEQ_PLAIN, 3)
-SEQ_INST(hat_attnseq_f16_d3, f16, 3, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_f16_d4, f16, 4, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_f16_d1_bias, f16, 1, 1, 2, SEQ_BIAS, 3)
-SEQ_INST(hat_attnseq_f16_d2_bias, f16, 2, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f16_d3_bias, f16, 3, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f16_d4_bias, f16, 4, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_f16_d1_cap, f16, 1, 1, 2, SEQ_CAP, 3)
-SEQ_INST(hat_attnseq_f16_d2_cap, f16, 2, 1, 2, SEQ_CAP, 3)
-SEQ_INST(hat_attnseq_f16_d3_cap, f16, 3, 1, 2, SEQ_CAP, 2)
-SEQ_INST(hat_attnseq_f16_d4_cap, f16, 4, 1, 2, SEQ_CAP, 2)
-SEQ_INST(hat_attnseq_f16_d1_both, f16, 1, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f16_d2_both, f16, 2, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f16_d3_both, f16, 3, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_f16_d4_both, f16, 4, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_bf16_d1, bf16, 1, 1, 2, SEQ_PLAIN, 3)
-SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 1, 2, SEQ_PLAIN, 3)
-SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 1, 2, SEQ_PLAIN, 2)
-SEQ_INST(hat_attnseq_bf16_d1_bias, bf16, 1, 1, 2, SEQ_BIAS, 3)
-SEQ_INST(hat_attnseq_bf16_d2_bias, bf16, 2, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_bf16_d3_bias, bf16, 3, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_bf16_d4_bias, bf16, 4, 1, 2, SEQ_BIAS, 2)
-SEQ_INST(hat_attnseq_bf16_d1_cap, bf16, 1, 1, 2, SEQ_CAP, 3)
-SEQ_INST(hat_attnseq_bf16_d2_cap, bf16, 2, 1, 2, SEQ_CAP, 3)
-SEQ_INST(hat_attnseq_bf16_d3_cap, bf16, 3, 1, 2, SEQ_CAP, 2)
-SEQ_INST(hat_attnseq_bf16_d4_cap, bf16, 4, 1, 2, SEQ_CAP, 2)
-SEQ_INST(hat_attnseq_bf16_d1_both, bf16, 1, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_bf16_d2_both, bf16, 2, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_bf16_d3_both, bf16, 3, 1, 2, SEQ_BOTH, 2)
-SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d1, f16, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_f16_d2, f16, 2, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_f16_d3, f16, 3, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f16_d4, f16, 4, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_f16_d1_bias, f16, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_f16_d2_bias, f16, 2, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f16_d3_bias, f16, 3, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f16_d4_bias, f16, 4, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_f16_d1_cap, f16, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_f16_d2_cap, f16, 2, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_f16_d3_cap, f16, 3, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_f16_d4_cap, f16, 4, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_f16_d1_both, f16, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d2_both, f16, 2, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d3_both, f16, 3, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_f16_d4_both, f16, 4, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d1, bf16, 1, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_bf16_d2, bf16, 2, 2, SEQ_PLAIN, 3)
+SEQ_INST(hat_attnseq_bf16_d3, bf16, 3, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_bf16_d4, bf16, 4, 2, SEQ_PLAIN, 2)
+SEQ_INST(hat_attnseq_bf16_d1_bias, bf16, 1, 2, SEQ_BIAS, 3)
+SEQ_INST(hat_attnseq_bf16_d2_bias, bf16, 2, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_bf16_d3_bias, bf16, 3, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_bf16_d4_bias, bf16, 4, 2, SEQ_BIAS, 2)
+SEQ_INST(hat_attnseq_bf16_d1_cap, bf16, 1, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_bf16_d2_cap, bf16, 2, 2, SEQ_CAP, 3)
+SEQ_INST(hat_attnseq_bf16_d3_cap, bf16, 3, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_bf16_d4_cap, bf16, 4, 2, SEQ_CAP, 2)
+SEQ_INST(hat_attnseq_bf16_d1_both, bf16, 1, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d2_both, bf16, 2, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d3_both, bf16, 3, 2, SEQ_BOTH, 2)
+SEQ_INST(hat_attnseq_bf16_d4_both, bf16, 4, 2, SEQ_BOTH, 2)
 #define SEQ_FP_INST(NAME, DT, KT, MODE, WPS)                                                                   \
     extern "C" __global__ __launch_bounds__(256, WPS) void NAME(SeqAttnArgs p)                               \
     {                                                                                                        \
